@@ -6,7 +6,8 @@ Session / Program / Executable lowering contract.
 """
 from ._lib import lib as native_library  # noqa: F401
 from .core import AffonError, Executable, FormalTensor, Program, Session, Tensor, TensorSpec, program  # noqa: F401
+from . import paged  # noqa: F401
 from .ops import add, quantized_matmul, slice, transpose  # noqa: F401
 
 __all__ = ["AffonError", "Executable", "FormalTensor", "Program", "Session", "Tensor", "TensorSpec", "program",
-           "quantized_matmul", "add", "slice", "transpose", "native_library"]
+           "quantized_matmul", "add", "slice", "transpose", "paged", "native_library"]

@@ -45,6 +45,24 @@ class AttnDesc(ctypes.Structure):
                 ("ld_out", c_i64)]
 
 
+class PagedDesc(ctypes.Structure):
+    _fields_ = [("struct_size", c_u32), ("seqs", c_i32), ("rows", c_i32), ("max_nodes", c_i32), ("kv_heads", c_i32),
+                ("head_dim", c_i32), ("page_size", c_i32), ("mask_words", c_i32), ("pages", c_i64),
+                ("page_stride", c_i64), ("head_stride", c_i64), ("token_stride", c_i64), ("ld_table", c_i64)]
+
+
+class AppendDesc(ctypes.Structure):
+    _fields_ = [("struct_size", c_u32), ("x_dtype", c_i32), ("rope", c_i32), ("q_heads", c_i32), ("q_offset", c_i32),
+                ("k_offset", c_i32), ("v_offset", c_i32), ("table_rows", c_i32), ("ld_qkv", c_i64), ("ld_q", c_i64)]
+
+
+class TreeAttnDesc(ctypes.Structure):
+    _fields_ = [("struct_size", c_u32), ("q_heads", c_i32), ("scale", ctypes.c_float), ("out_pair_order", c_i32),
+                ("ld_q", c_i64), ("ld_out", c_i64)]
+
+
+ROPE = {"none": 0, "half": 1, "interleaved": 2}
+MAX_TREE_NODES = 256  # most new tokens of one sequence in a paged step
 EPI_STORE, EPI_RESID, EPI_SILU_MUL, EPI_ARGMAX, EPI_RESID_AR = 0, 1, 2, 3, 4
 SS_WIDTH = 32      # row width of the per-16-column sums of squares ([cols/16][SS_WIDTH] f32)
 MAX_QMV_ROWS = 32  # activation rows the decode qmv takes in one pass
@@ -99,6 +117,12 @@ SIGNATURES = {
     "affon_b200_embed": ([c_vp, c_vp, c_i64, c_i64, c_vp, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp, c_i64, c_i32],
                          c_i32),
     "affon_b200_argmax_finalize": ([c_vp, c_vp, c_i32, c_vp, c_vp, c_i32, c_vp, c_vp], c_i32),
+    "affon_b200_paged_validate": ([ctypes.POINTER(PagedDesc)], c_i32),
+    "affon_b200_paged_plan": ([c_vp, ctypes.POINTER(PagedDesc)] + [c_vp] * 7, c_i32),
+    "affon_b200_paged_append": ([c_vp, ctypes.POINTER(PagedDesc), ctypes.POINTER(AppendDesc)] + [c_vp] * 8, c_i32),
+    "affon_b200_tree_attention": ([c_vp, ctypes.POINTER(PagedDesc), ctypes.POINTER(TreeAttnDesc)] + [c_vp] * 8, c_i32),
+    "affon_b200_tree_accept": ([c_vp, ctypes.POINTER(PagedDesc), c_i32, c_i64] + [c_vp] * 10 + [c_i64, c_vp, c_vp],
+                               c_i32),
     "affon_b200_launch_count": ([], ctypes.c_uint64),
 }
 

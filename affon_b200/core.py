@@ -201,6 +201,14 @@ class Session:
                                           ctypes.byref(sel) if sel is not None else None)
         check(status, "quantized_matmul")
 
+    def synchronize(self):
+        """Wait for the stream of the Session's last launch and raise what the kernels reported since the last
+        check: `timeout` (a bounded wait gave up) or `invalid_arg` (a length, index, position or token in device
+        memory that does not fit its buffer)."""
+        if self.disposed:
+            raise AffonError("invalid_arg", "Session has been disposed")
+        check(_lib.lib().affon_b200_ctx_synchronize(self._ctx), "Session")
+
     def dispose(self):
         if not self.disposed:
             for exe in self._cache.values():

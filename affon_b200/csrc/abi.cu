@@ -40,19 +40,7 @@ int cuda_fail(cudaError_t e, const char *what) {
 
 constexpr size_t kDefaultWorkspace = size_t(64) << 20;
 
-// Makes ctx->device current for the scope of one call.
-struct DeviceGuard {
-    int prev = -1;
-    bool ok = true;
-    explicit DeviceGuard(int dev) {
-        if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
-        if (prev != dev) ok = cudaSetDevice(dev) == cudaSuccess;
-    }
-    ~DeviceGuard() {
-        int cur = -1;
-        if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
-    }
-};
+using afb::DeviceGuard;
 
 int env_device() {
     const char *v = getenv("AFFON_CUDA_DEVICE");

@@ -151,6 +151,49 @@ cudaError_t launch_embed(const void *table, int64_t ld_table, int64_t vocab, con
 cudaError_t launch_finalize(const unsigned long long *amax, int B, int *tokens, int *history, int history_rows,
                             int *pos, int *step, cudaStream_t stream, bool pdl);
 
+// Paged cache and drafted trees (paged.cu, tree_attention.cu).  Device-side
+// lengths, tables and indices are checked by the kernels, which report
+// DEV_BOUNDS in the workspace's status word.
+constexpr int kMaxTreeNodes = 256;
+struct PagedShape {
+    int seqs, rows, max_nodes, kv_heads, head_dim, page_shift, mask_words;
+    int64_t pages, page_stride, head_stride, token_stride, ld_table;
+};
+struct PagedStep {  // the device arrays of one step
+    const int *cu_nodes, *parents, *ctx_lens, *page_table;
+};
+cudaError_t launch_paged_plan(const PagedShape &s, const PagedStep &t, int *positions, int *slots, uint32_t *mask,
+                              void *workspace, cudaStream_t stream, bool pdl);
+struct AppendArgs {
+    const void *qkv;
+    const float *cos_t, *sin_t;
+    const int *positions, *slots;
+    uint16_t *q_out, *k_cache, *v_cache;
+    int x_f32, rope, q_heads, q_off, k_off, v_off, table_rows;
+    int64_t ld_qkv, ld_q;
+};
+cudaError_t launch_paged_append(const PagedShape &s, const AppendArgs &a, void *workspace, cudaStream_t stream,
+                                bool pdl);
+struct TreeAttnArgs {
+    const uint16_t *q, *k_cache, *v_cache;
+    uint16_t *out;
+    const uint32_t *mask;  // null: chains
+    int q_heads, out_pair_order;
+    float scale;
+    int64_t ld_q, ld_out;
+};
+cudaError_t launch_tree_attention(const PagedShape &s, const PagedStep &t, const TreeAttnArgs &a, void *workspace,
+                                  int num_sms, cudaStream_t stream, bool pdl);
+struct AcceptArgs {
+    const int *tokens, *predicted;
+    uint16_t *k_cache, *v_cache;
+    int layers;
+    int64_t layer_stride, ld_path;
+    int *counts, *path, *next_tokens, *lens_out;
+};
+cudaError_t launch_tree_accept(const PagedShape &s, const PagedStep &t, const AcceptArgs &a, void *workspace,
+                               cudaStream_t stream, bool pdl);
+
 // Prefill qmm on tcgen05 tensor cores (M >= 64), bf16 x/s/b, 4/8-bit, group 64.
 bool qmm_tc_supported(const QmmArgs &a, const char **why);
 cudaError_t launch_qmm_tc(const QmmArgs &a, void *workspace, cudaStream_t stream);
@@ -166,6 +209,20 @@ cudaError_t launch_qmm_exact(const QmmArgs &a, void *workspace, size_t workspace
 void qmm_exact_set_slice_cap(int64_t rows);  // test hook: most rows per pass (0 = workspace bound)
 
 void count_launch(uint64_t n = 1);
+
+// Makes ctx->device current for the scope of one call.
+struct DeviceGuard {
+    int prev = -1;
+    bool ok = true;
+    explicit DeviceGuard(int dev) {
+        if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
+        if (prev != dev) ok = cudaSetDevice(dev) == cudaSuccess;
+    }
+    ~DeviceGuard() {
+        int cur = -1;
+        if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
+    }
+};
 
 }  // namespace afb
 

@@ -325,6 +325,127 @@ int affon_b200_argmax_finalize(affon_b200_ctx *ctx, const unsigned long long *am
                                int *history, int history_rows, int *pos, int *step);
 
 /* ---------------------------------------------------------------------------
+ * Paged key/value cache and drafted trees.  No counterpart in the reference,
+ * whose models use a fixed-capacity cache (docs of its models: apertus-8b.md:16);
+ * these let sequences of different lengths share one pool and let one step
+ * verify several drafted tokens per sequence.
+ *
+ * A cache is two pools (keys, values) of `pages` pages, each holding
+ * `page_size` positions of every KV head: element (page, head, position, dim)
+ * lies at page*page_stride + head*head_stride + position*token_stride + dim.
+ * Row s of page_table lists sequence s's pages in order; pages may be shared
+ * between sequences as long as no step appends into a shared one.
+ *
+ * A step is a ragged batch: rows cu_nodes[s] .. cu_nodes[s+1]-1 of its buffers
+ * are the new tokens ("nodes") of sequence s, which already holds ctx_lens[s]
+ * positions; node i takes cache position ctx_lens[s]+i.  The nodes of a
+ * sequence form a forest: parents[row] is the index, within the sequence, of
+ * the node it continues (always a lower index), or negative for a root.  A
+ * sequence may have no nodes, and rows outside [cu_nodes[0], cu_nodes[seqs])
+ * are padding.  One node per sequence is plain decoding; parents == NULL makes
+ * every node continue the one before it (a chunk of a prompt).
+ *
+ * All lengths, tables and indices live in device memory and are checked by
+ * the kernels: a sequence whose lengths do not fit (cu_nodes not ascending or
+ * beyond `rows`, more than max_nodes nodes, a negative length, more positions
+ * than its page-table row) is skipped, its outputs are left as they were
+ * (affon_b200_paged_plan marks its rows as padding), and the next
+ * affon_b200_ctx_synchronize returns AFFON_B200_INVALID_ARG; so does a page
+ * outside the pool, whose positions read as zero and are never written. */
+typedef struct affon_b200_paged_desc {
+    uint32_t struct_size;
+    int32_t seqs;        /* 1..65536 */
+    int32_t rows;        /* rows of the step's buffers */
+    int32_t max_nodes;   /* most nodes of one sequence, 1..256 */
+    int32_t kv_heads;    /* 1..1024 */
+    int32_t head_dim;    /* 64 or 128 */
+    int32_t page_size;   /* 16, 32, 64, 128 or 256 */
+    int32_t mask_words;  /* 32-bit words per row of the mask: ceil(max_nodes/32) at least, at most 8 */
+    int64_t pages;       /* pages*page_size < 2^31 */
+    int64_t page_stride, head_stride, token_stride; /* elements; multiples of 8, token_stride >= head_dim */
+    int64_t ld_table;    /* pages per row of page_table; ld_table*page_size < 2^31 */
+} affon_b200_paged_desc;
+
+/* The descriptor's own rules (no GPU call). */
+int affon_b200_paged_validate(const affon_b200_paged_desc *desc);
+
+/* The plan of a step, computed once and used by every layer: per row the
+ * rotation position (ctx_lens[s] plus the node's depth in its tree), the slot
+ * (page*page_size + position in the page; -1 for padding) and the mask (bit j
+ * of word j/32 set when node j is the row's node or one of its ancestors).
+ * A parent that is not a lower index is reported like a bad length and its
+ * node becomes a root.  Padding rows get position 0, slot -1, mask 0. */
+int affon_b200_paged_plan(affon_b200_ctx *ctx, const affon_b200_paged_desc *desc, const int *cu_nodes,
+                          const int *parents, const int *ctx_lens, const int *page_table, int *positions, int *slots,
+                          uint32_t *mask);
+
+typedef enum affon_b200_rope {
+    AFFON_B200_ROPE_NONE = 0,
+    AFFON_B200_ROPE_HALF = 1,       /* pairs (d, d + head_dim/2), as affon_b200_decode_attention */
+    AFFON_B200_ROPE_INTERLEAVED = 2 /* pairs (2d, 2d + 1) */
+} affon_b200_rope;
+
+/* Rotate and append: for every row with slot >= 0, the queries (q_heads heads
+ * from column q_offset) and keys (kv_heads heads from k_offset) of qkv's row
+ * are rotated by the row's position (tables [table_rows][head_dim/2] f32; the
+ * products and their sum in f32, rounded once to bf16), queries go to
+ * q_out[row] and keys and values (from v_offset) to the row's slot.  qkv is
+ * f32 or bf16; q_heads may be 0 (q_out unused).  A position outside the tables
+ * or a slot outside the pool skips the row and is reported like a bad length.
+ * Two rows of one call must not share a slot. */
+typedef struct affon_b200_append_desc {
+    uint32_t struct_size;
+    int32_t x_dtype;     /* AFFON_B200_F32 or AFFON_B200_BF16 */
+    int32_t rope;        /* affon_b200_rope */
+    int32_t q_heads;
+    int32_t q_offset, k_offset, v_offset;
+    int32_t table_rows;
+    int64_t ld_qkv, ld_q;
+} affon_b200_append_desc;
+
+int affon_b200_paged_append(affon_b200_ctx *ctx, const affon_b200_paged_desc *desc, const affon_b200_append_desc *a,
+                            const void *qkv, const float *rope_cos, const float *rope_sin, const int *positions,
+                            const int *slots, void *q_out, void *k_cache, void *v_cache);
+
+/* Attention of the step's nodes over the paged cache: query head h of a row
+ * reads KV head h / (q_heads / kv_heads), attends to its sequence's first
+ * ctx_lens[s] positions and to the drafted positions its mask names (NULL: the
+ * nodes up to its own), and writes softmax(scale * q.k) v as bf16.  q and out
+ * are bf16 [rows][q_heads*head_dim].  A row that sees nothing gets zeros;
+ * padding rows are left as they were.  What a mask hides does not reach the
+ * result, infinities and NaN included.  out must not overlap q or the caches.
+ * The launch uses the context's workspace. */
+typedef struct affon_b200_tree_attn_desc {
+    uint32_t struct_size;
+    int32_t q_heads;        /* a multiple of kv_heads */
+    float scale;
+    int32_t out_pair_order; /* write the output in 4-bit qmv pair order */
+    int64_t ld_q, ld_out;
+} affon_b200_tree_attn_desc;
+
+int affon_b200_tree_attention(affon_b200_ctx *ctx, const affon_b200_paged_desc *desc,
+                              const affon_b200_tree_attn_desc *a, const void *q, const int *cu_nodes,
+                              const int *ctx_lens, const int *page_table, const uint32_t *mask, const void *k_cache,
+                              const void *v_cache, void *out);
+
+/* Greedy acceptance of the drafted trees after a verification step:
+ * predicted[row] is the model's next token after that row's node.  Node 0 of a
+ * sequence is its last sampled token and is always accepted; from an accepted
+ * node the walk goes on to its lowest-index child whose token is the predicted
+ * one, until there is none.  Writes per sequence counts[s] (accepted nodes),
+ * path[s*ld_path + i] (their indices, -1 behind the last, max_nodes entries),
+ * next_tokens[s] (predicted at the last accepted node) and lens_out[s] =
+ * ctx_lens[s] + counts[s]; and moves the accepted nodes' keys and values
+ * together, from position ctx_lens[s]+path[i] to ctx_lens[s]+i, in `layers`
+ * caches that lie layer_stride elements apart.  A sequence without nodes gets
+ * count 0, next token -1 and keeps its length.  lens_out may be ctx_lens.
+ * parents == NULL: chains.  layers 0 moves nothing (the caches may be NULL). */
+int affon_b200_tree_accept(affon_b200_ctx *ctx, const affon_b200_paged_desc *desc, int layers, int64_t layer_stride,
+                           const int *cu_nodes, const int *parents, const int *tokens, const int *predicted,
+                           const int *page_table, const int *ctx_lens, void *k_cache, void *v_cache, int *counts,
+                           int *path, int64_t ld_path, int *next_tokens, int *lens_out);
+
+/* ---------------------------------------------------------------------------
  * Tensor parallelism (whole-model decode sharded over the GPUs of one node,
  * one process per GPU).  No counterpart in the reference, which has no
  * multi-device contract (docs/core/backend-support.md:82); the sharding is
