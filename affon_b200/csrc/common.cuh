@@ -24,6 +24,13 @@ AFB_DEVICE uint32_t pack_bf16x2(float lo, float hi) {
     return r;
 }
 
+// 2^x, one ex2.approx (subnormal results are zero; 2^-inf = 0).
+AFB_DEVICE float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // (x0, x1) as bf16 pairs hi = bf16(x) and lo = bf16(x - hi): hi + lo carries
 // ~16 significant bits of x.
 AFB_DEVICE void split_bf16x2(float x0, float x1, uint32_t &hi, uint32_t &lo) {

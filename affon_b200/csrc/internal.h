@@ -182,6 +182,7 @@ struct TreeAttnArgs {
     float scale;
     int64_t ld_q, ld_out;
 };
+size_t tree_attention_workspace_bytes(int head_dim, int num_sms);
 cudaError_t launch_tree_attention(const PagedShape &s, const PagedStep &t, const TreeAttnArgs &a, void *workspace,
                                   int num_sms, cudaStream_t stream, bool pdl);
 struct AcceptArgs {

@@ -160,6 +160,8 @@ int affon_b200_tree_attention(affon_b200_ctx *ctx, const affon_b200_paged_desc *
         return fail(AFFON_B200_INVALID_ARG, "tree_attention: null buffer");
     if (!al16(q) || !al16(k_cache) || !al16(v_cache) || !al16(out))
         return fail(AFFON_B200_INVALID_ARG, "tree_attention: buffers must be 16-byte aligned");
+    if (afb::tree_attention_workspace_bytes(s.head_dim, ctx->num_sms) > ctx->workspace_bytes)
+        return fail(AFFON_B200_UNSUPPORTED, "tree_attention: partial results exceed the context workspace");
     afb::TreeAttnArgs a{};
     a.q = static_cast<const uint16_t *>(q);
     a.k_cache = static_cast<const uint16_t *>(k_cache);

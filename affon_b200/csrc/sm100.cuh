@@ -111,6 +111,21 @@ AFB_DEVICE void tma_load_2d_hint(void *smem_dst, const CUtensorMap *map, uint64_
         "l"(policy)
         : "memory");
 }
+// 4D tiled TMA load with an L2 cache policy.
+AFB_DEVICE void tma_load_4d_hint(void *smem_dst, const CUtensorMap *map, uint64_t *bar, int c0, int c1, int c2, int c3,
+                                 uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+        " [%0], [%1, {%3, %4, %5, %6}], [%2], %7;"
+        ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2),
+        "r"(c3), "l"(policy)
+        : "memory");
+}
+AFB_DEVICE uint64_t l2_evict_normal() {
+    uint64_t policy;
+    asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(policy));
+    return policy;
+}
 // L2 policy for data read once per launch (streamed weights, caches): its
 // lines are the first evicted, so streaming does not push out what the
 // surrounding kernels reuse.
@@ -178,6 +193,21 @@ AFB_DEVICE uint64_t umma_desc_sw128(uint32_t smem_addr) {
     return d;
 }
 
+// The same for an operand whose M or N axis is contiguous (MN-major): 64
+// elements (128 B) per row of the K axis, 8-row atoms of 1024 B along K
+// (stride byte offset), `mn_bytes` between runs of 64 M or N elements (leading
+// byte offset).  A 16-element K step is 2048 B.
+AFB_DEVICE uint64_t umma_desc_mn_sw128(uint32_t smem_addr, uint32_t mn_bytes) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu);
+    d |= static_cast<uint64_t>(mn_bytes >> 4) << 16;
+    d |= static_cast<uint64_t>(1024u >> 4) << 32;
+    d |= static_cast<uint64_t>(1u) << 46;
+    d |= static_cast<uint64_t>(2u) << 61;
+    return d;
+}
+constexpr uint32_t kUmmaTransposeB = 1u << 16;  // instruction descriptor: B is MN-major
+
 // Instruction descriptor, kind::f16: bf16 A and B, f32 accumulate, both
 // operands K-major, M x N tile.
 __host__ __device__ constexpr uint32_t umma_idesc_bf16(int M, int N) {
@@ -194,6 +224,16 @@ AFB_DEVICE void umma_bf16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, 
         "setp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
         ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// A from tensor memory: lane = row, a 32-bit column = two consecutive K elements.
+AFB_DEVICE void umma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
         : "memory");
 }
 
@@ -221,6 +261,26 @@ AFB_DEVICE void tmem_ld_32x32b_x32(uint32_t taddr, uint32_t (&r)[32]) {
           "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(taddr));
+}
+// 16 and 32 consecutive columns per thread into tensor memory.
+AFB_DEVICE void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+            taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+AFB_DEVICE void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// Makes every later use of r depend on this point of the (volatile) asm
+// sequence: after tmem_wait_ld(), for registers of a pending load.
+AFB_DEVICE void tie_regs(uint32_t (&r)[32]) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 16)
+        asm volatile(""
+                     : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]),
+                       "+r"(r[i + 6]), "+r"(r[i + 7]), "+r"(r[i + 8]), "+r"(r[i + 9]), "+r"(r[i + 10]), "+r"(r[i + 11]),
+                       "+r"(r[i + 12]), "+r"(r[i + 13]), "+r"(r[i + 14]), "+r"(r[i + 15]));
 }
 AFB_DEVICE void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 // The same wait, with the 16 registers of a pending tmem_ld_32x32b_x16 as
@@ -253,6 +313,10 @@ const CUtensorMap *cached_tensor_map_2d(CUtensorMapDataType dtype, const void *b
 const CUtensorMap *cached_tensor_map_3d(CUtensorMapDataType dtype, const void *base, uint64_t d0, uint64_t d1,
                                         uint64_t d2, uint64_t stride1_bytes, uint64_t stride2_bytes, uint32_t b0,
                                         uint32_t b1, uint32_t b2, CUtensorMapSwizzle swizzle);
+// A 4D map (dims and boxes innermost first, byte strides of dims 1 to 3), for
+// callers that encode one per launch.
+bool encode_tensor_map_4d(CUtensorMap *map, CUtensorMapDataType dtype, const void *base, const uint64_t (&dims)[4],
+                          const uint64_t (&strides)[3], const uint32_t (&box)[4], CUtensorMapSwizzle swizzle);
 // cudaFuncSetAttribute(MaxDynamicSharedMemorySize) once per (kernel, device, size).
 cudaError_t ensure_smem_attr(const void *kernel, int bytes);
 

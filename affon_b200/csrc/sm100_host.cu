@@ -38,6 +38,19 @@ bool encode_tensor_map_2d(CUtensorMap *map, CUtensorMapDataType dtype, const voi
     return r == CUDA_SUCCESS;
 }
 
+bool encode_tensor_map_4d(CUtensorMap *map, CUtensorMapDataType dtype, const void *base, const uint64_t (&dims)[4],
+                          const uint64_t (&strides)[3], const uint32_t (&box)[4], CUtensorMapSwizzle swizzle) {
+    auto fn = encode_fn();
+    if (!fn) return false;
+    cuuint64_t d[4], st[3];
+    cuuint32_t b[4], estr[4] = {1, 1, 1, 1};
+    for (int i = 0; i < 4; ++i) d[i] = dims[i], b[i] = box[i];
+    for (int i = 0; i < 3; ++i) st[i] = strides[i];
+    CUresult r = fn(map, dtype, 4, const_cast<void *>(base), d, st, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS;
+}
+
 namespace {
 using MapKey = std::tuple<int, uintptr_t, uint64_t, uint64_t, uint64_t, uint32_t, uint32_t, int>;
 struct MapCache {
