@@ -149,8 +149,8 @@ int affon_b200_tree_attention(affon_b200_ctx *ctx, const affon_b200_paged_desc *
         return fail(AFFON_B200_INVALID_ARG, "tree_attention: null context or bad descriptor");
     if (d->q_heads < 1 || d->q_heads > 65536 || d->q_heads % s.kv_heads)
         return fail(AFFON_B200_INVALID_SHAPE, "tree_attention: q_heads must be a multiple of kv_heads, at most 65536");
-    if (!(d->scale > -3.0e38f && d->scale < 3.0e38f))
-        return fail(AFFON_B200_INVALID_ARG, "tree_attention: scale must be finite");
+    if (!(d->scale > -3.0e38f && d->scale < 3.0e38f) || d->scale == 0.0f)
+        return fail(AFFON_B200_INVALID_ARG, "tree_attention: scale must be finite and not zero");
     const int64_t cols = int64_t(d->q_heads) * s.head_dim;
     if (d->ld_q < cols || d->ld_out < cols || d->ld_q % 8 || d->ld_out % 8)
         return fail(AFFON_B200_INVALID_SHAPE, "tree_attention: ld_q and ld_out must be multiples of 8 and hold q_heads "

@@ -206,7 +206,8 @@ AFB_DEVICE uint64_t umma_desc_mn_sw128(uint32_t smem_addr, uint32_t mn_bytes) {
     d |= static_cast<uint64_t>(2u) << 61;
     return d;
 }
-constexpr uint32_t kUmmaTransposeB = 1u << 16;  // instruction descriptor: B is MN-major
+// Instruction descriptor bits: B is MN-major; A enters negated.
+constexpr uint32_t kUmmaTransposeB = 1u << 16, kUmmaNegateA = 1u << 13;
 
 // Instruction descriptor, kind::f16: bf16 A and B, f32 accumulate, both
 // operands K-major, M x N tile.

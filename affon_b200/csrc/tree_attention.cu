@@ -16,16 +16,23 @@
 // the workspace and the CTAs that share a unit merge it together at the end,
 // each a share of its rows, in piece order (results do not depend on timing).
 //
-// Pipeline.  A producer warp brings K and V tiles page by page through a
-// shared-memory ring (TMA, 128-byte swizzle); an MMA warp issues S = Q K^T
-// (both from shared memory) and O += P V (P from tensor memory, V read along
-// its dims); two warpgroups, a thread per row, turn S into P.  The two are two
-// streams with their own S, O, maximum and sum: units of more than 128 rows
-// give each its own 128 rows and both take every tile; smaller units give both
-// the same rows and they take alternate tiles, merged when the unit ends.
-// While one stream is in its softmax the tensor cores work for the other.
+// Roles.  A scheduler warp reads the lengths and queues the CTA's pieces; a
+// query warp copies their rows ahead of time; a producer warp brings K and V
+// tiles page by page through a shared-memory ring (TMA, 128-byte swizzle); an
+// MMA warp issues S = Q K^T (both from shared memory) and O += P V (P from
+// tensor memory, V read along its dims); two warpgroups, a thread per row,
+// turn S into P.  The two are two streams with their own S, O, maximum and
+// sum: units of more than 128 rows give each its own 128 rows and both take
+// every tile; smaller units give both the same rows and they take alternate
+// tiles.  While one stream is in its softmax the tensor cores work for the
+// other.  Units of at most 64 (16) rows fill the 128 rows of the MMA with 2
+// (4) copies, and each copy's warps take half (a quarter) of a tile's
+// positions: the softmax of few rows then runs on all warps.  The streams'
+// and copies' results are joined when the piece ends.
+//
 // A row's maximum is only raised (and O rescaled) when it grows by more than
-// 2^8, so O is rarely touched.
+// 2^8, so O is rarely touched.  The loops over a tile's columns and a row's
+// dims stay rolled: code that runs once per launch is bound by its fetching.
 //
 // Rounding: P is rounded to bf16 for the tensor cores (as V is bf16, it is the
 // smaller part of the result's own rounding); the sum l adds the rounded
@@ -44,13 +51,11 @@ namespace tattn {
 constexpr int TILE = 128;           // positions per tile
 constexpr int ROWS = 256;           // query rows of a unit, at most
 constexpr int SOFTMAX_WARPS = 8;    // two warpgroups
-constexpr int PRODUCER = 8, MMA = 9;
-constexpr int THREADS = 32 * 12;    // the last two warps only complete a warpgroup
-// Registers per thread: 168 at launch, moved from the third warpgroup to the
-// two softmax ones, whose threads hold a row of 128 scores.
-constexpr int LAUNCH_REGS = 168, SOFTMAX_REGS = 208, OTHER_REGS = 88;
-static_assert(2 * SOFTMAX_REGS + OTHER_REGS <= 3 * LAUNCH_REGS, "register split exceeds the launch allocation");
+constexpr int PRODUCER = 8, MMA = 9, SCHEDULER = 10, QUERIES = 11;
+constexpr int THREADS = 32 * 12;
+constexpr int SOFTMAX_THREADS = 32 * SOFTMAX_WARPS;
 constexpr int HALF_BYTES = TILE * 128;  // 64 dims of a tile
+constexpr int PIECES = 4;           // pieces queued ahead
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float RAISE = 8.0f;       // log2: how far scores may pass the running maximum before it is raised
 
@@ -72,12 +77,6 @@ struct Params {
     unsigned *arrived, *done, *status;
 };
 
-// Where a CTA's share of the tiles begins.
-struct Share {
-    int64_t begin, end, total, at;  // at: `begin`'s offset within its sequence
-    int seq, grid;
-};
-
 // The tiles of one sequence: kv_heads * row tiles * position tiles.
 struct SeqTiles {
     SeqSpan sp;
@@ -93,90 +92,42 @@ __device__ __forceinline__ SeqTiles seq_tiles(const Params &p, int seq) {
     return r;
 }
 
-// Computed by one warp.
-__device__ __forceinline__ void find_share(const Params &p, Share *out) {
-    const int lane = threadIdx.x & 31;
-    int64_t total = 0;
-    for (int base = 0; base < p.s.seqs; base += 32) {
-        int64_t mine = 0;
-        if (base + lane < p.s.seqs) {
-            const SeqTiles q = seq_tiles(p, base + lane);
-            mine = q.tiles(p.s.kv_heads);
-            if (!q.sp.ok && blockIdx.x == 0) atomicExch(p.status, static_cast<unsigned>(DEV_BOUNDS));
-        }
-#pragma unroll
-        for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-        total += mine;
+// The division of all tiles over the grid: the first `extra` CTAs take
+// per + 1, the others per.
+struct Shares {
+    int grid, per, extra;
+    __device__ __forceinline__ int begin(int cta) const { return cta * per + min(cta, extra); }
+    __device__ __forceinline__ int owner(int tile) const {
+        const int big = extra * (per + 1);
+        return tile < big ? tile / (per + 1) : extra + (tile - big) / per;
     }
-    Share r{};
-    r.total = total;
-    r.grid = static_cast<int>(total < gridDim.x ? total : gridDim.x);
-    if (static_cast<int>(blockIdx.x) < r.grid) {
-        r.begin = blockIdx.x * total / r.grid;
-        r.end = (blockIdx.x + 1) * total / r.grid;
-        int64_t before = 0;
-        for (int base = 0; base < p.s.seqs; base += 32) {
-            const int64_t mine = base + lane < p.s.seqs ? seq_tiles(p, base + lane).tiles(p.s.kv_heads) : 0;
-            int64_t upto = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += v;
-            }
-            const unsigned past = __ballot_sync(0xffffffffu, before + upto > r.begin);
-            if (past) {
-                const int l = __ffs(past) - 1;
-                r.seq = base + l;
-                r.at = r.begin - before - __shfl_sync(0xffffffffu, upto - mine, l);
-                break;
-            }
-            before += __shfl_sync(0xffffffffu, upto, 31);
-        }
-    }
-    if (lane == 0) *out = r;
-}
-// The CTA whose share holds tile x.
-__device__ __forceinline__ int owner(const Share &sh, int64_t x) {
-    return static_cast<int>(((x + 1) * sh.grid - 1) / sh.total);
-}
+};
 
-// A piece of a unit: tiles [t0, t1) of nt.
+// A piece of a unit: tiles [t0, t1) of nt.  rows 0 ends the queue.
 struct Piece {
     int seq, first, n, ctx, kv, row0, rows, t0, t1, nt;
-    int64_t start;  // the unit's first tile in the order of all tiles
+    int start;       // the unit's first tile in the order of all tiles
+    int owner0, ctas;  // the CTAs that share the unit
     __device__ __forceinline__ bool both() const { return rows > TILE; }  // two row tiles, every position tile for both
     __device__ __forceinline__ int items() const { return both() ? 2 * (t1 - t0) : t1 - t0; }
+    // log2 of the copies of the rows in the 128 rows of the MMA: a copy's
+    // results are joined through the piece's own query buffer, which holds
+    // 64 + 64 rows of f32, or 3 x 16.
+    __device__ __forceinline__ int copies() const { return rows <= 16 ? 2 : rows <= 64 ? 1 : 0; }
 };
-struct Walk {
-    int64_t pos, end, at;
-    int seq;
-    SeqTiles q;
-    __device__ __forceinline__ Walk(const Params &p, const Share &sh) : pos(sh.begin), end(sh.end), at(sh.at), seq(sh.seq) {
-        if (pos < end) q = seq_tiles(p, seq);
+
+// Which of the two query buffers a piece uses and how often each was used.
+struct QuerySlots {
+    unsigned used[2] = {0u, 0u};
+    int next = 0;
+    __device__ __forceinline__ int take(bool both) {
+        const int s = both ? 0 : next;
+        next = both ? 0 : next ^ 1;
+        ++used[s];
+        if (both) ++used[1];
+        return s;
     }
-    __device__ __forceinline__ bool next(const Params &p, Piece &d) {
-        if (pos >= end) return false;
-        while (at >= q.tiles(p.s.kv_heads)) {
-            at = 0;
-            q = seq_tiles(p, ++seq);
-        }
-        const int64_t unit = at / q.nt;
-        d.seq = seq;
-        d.first = q.sp.first;
-        d.n = q.n;
-        d.ctx = q.sp.ctx;
-        d.nt = q.nt;
-        d.t0 = static_cast<int>(at - unit * q.nt);
-        const int64_t left = end - pos;
-        d.t1 = left < q.nt - d.t0 ? d.t0 + static_cast<int>(left) : q.nt;
-        d.kv = static_cast<int>(unit / q.units);
-        d.row0 = static_cast<int>(unit % q.units) * ROWS;
-        d.rows = min(ROWS, q.n * p.group - d.row0);
-        d.start = pos - d.t0;
-        pos += d.t1 - d.t0;
-        at += d.t1 - d.t0;
-        return true;
-    }
+    __device__ __forceinline__ uint32_t parity(int slot) const { return (used[slot] - 1) & 1; }  // of its current use
 };
 
 // 32 visibility bits of a row, for drafted nodes j0 .. j0+31 (cached
@@ -203,21 +154,38 @@ __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volati
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, status) && !*abort);
 }
 
-template <int N>
-__device__ __forceinline__ void store_out(uint16_t *dst, const float (&x)[N], int pair_order) {
-#pragma unroll
-    for (int i = 0; i < N; i += 8) {
-        uint4 u;
-        if (pair_order)
-            u = make_uint4(pack_bf16x2(x[i], x[i + 4]), pack_bf16x2(x[i + 1], x[i + 5]), pack_bf16x2(x[i + 2], x[i + 6]),
-                           pack_bf16x2(x[i + 3], x[i + 7]));
-        else
-            u = make_uint4(pack_bf16x2(x[i], x[i + 1]), pack_bf16x2(x[i + 2], x[i + 3]), pack_bf16x2(x[i + 4], x[i + 5]),
-                           pack_bf16x2(x[i + 6], x[i + 7]));
-        *reinterpret_cast<uint4 *>(dst + i) = u;
+// Copies 16 bytes to shared memory without registers (zeros when !take).
+__device__ __forceinline__ void copy16_async(void *dst, const void *src, bool take) {
+    const int bytes = take ? 16 : 0;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
+}
+
+// Infinities and NaN among the drafted values, which were kept from the
+// tensor cores, for a row that sees them: added to what the row's thread has
+// just stored (dims dim0 .. dim1-1; rec: f32 partial, out: bf16 result).
+__device__ __noinline__ void add_odd_values(const Params &p, const Piece &d, const RowMask &mask, const uint32_t *odd,
+                                            int dim0, int dim1, float *rec, uint16_t *out) {
+    for (int k = 0; k < kMaxTreeNodes / 32; ++k) {
+        for (uint32_t set = odd[k] ? odd[k] & mask.word(k) : 0u; set; set &= set - 1) {
+            const int pos = d.ctx + 32 * k + __ffs(set) - 1;
+            const int page = p.t.page_table[d.seq * p.s.ld_table + (pos >> p.s.page_shift)];
+            if (page < 0 || page >= p.s.pages) continue;
+            const uint16_t *src = p.a.v_cache + page * p.s.page_stride + d.kv * p.s.head_stride +
+                                  (pos & ((1 << p.s.page_shift) - 1)) * p.s.token_stride;
+            for (int dim = dim0; dim < dim1; ++dim) {
+                if ((src[dim] & 0x7F80u) != 0x7F80u) continue;
+                const float v = bf16_bits_to_f32(src[dim]);
+                if (rec) {
+                    rec[dim] += v;
+                } else {
+                    const int e = dim & 7;
+                    uint16_t *o = out + (p.a.out_pair_order ? (dim & ~7) + (e < 4 ? 2 * e : 2 * (e - 4) + 1) : dim);
+                    *o = f32_to_bf16_bits(bf16_bits_to_f32(*o) + v);
+                }
+            }
+        }
     }
 }
-__device__ __forceinline__ float finish(float o, float l) { return l == 0.0f ? 0.0f : o / l; }
 
 template <int HD>
 __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid_constant__ CUtensorMap kmap,
@@ -231,14 +199,17 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
     uint64_t *empty = full + C::STAGES;
     uint64_t *s_full = empty + C::STAGES;  // [2] scores of a stream are in tensor memory
     uint64_t *p_full = s_full + 2;         // [2] probabilities of a stream are
-    uint64_t *q_full = p_full + 2;
-    uint64_t *unit_done = q_full + 1;      // every MMA of the piece has ended
-    Share *share = reinterpret_cast<Share *>(unit_done + 1);
-    Piece *shared_units = reinterpret_cast<Piece *>(share + 1);  // [2] pieces of shared units: the end of one, the start of another
-    uint32_t *odd = reinterpret_cast<uint32_t *>(shared_units + 2);  // [8] drafted nodes whose values are not all finite
-    uint32_t *tmem_addr = odd + 8;
+    uint64_t *q_full = p_full + 2;         // [2] query buffers
+    uint64_t *q_empty = q_full + 2;
+    uint64_t *d_full = q_empty + 2;        // [PIECES] the queue
+    uint64_t *d_empty = d_full + PIECES;
+    uint64_t *unit_done = d_empty + PIECES;  // every MMA of the piece has ended
+    uint64_t *o_free = unit_done + 1;        // its O has been read
+    Piece *queue = reinterpret_cast<Piece *>(o_free + 1);
+    Piece *shared_units = queue + PIECES;    // [2] pieces of shared units: the end of one, the start of another
+    uint32_t *odd = reinterpret_cast<uint32_t *>(shared_units + 2);  // drafted nodes whose values are not all finite
+    uint32_t *tmem_addr = odd + kMaxTreeNodes / 32;
     volatile int *abort = reinterpret_cast<volatile int *>(tmem_addr + 1);
-    int *go = const_cast<int *>(abort) + 1;
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
@@ -249,9 +220,15 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 128);
+            mbar_init(&q_full[i], 1);
+            mbar_init(&q_empty[i], SOFTMAX_WARPS);
         }
-        mbar_init(q_full, 32 * SOFTMAX_WARPS);
+        for (int i = 0; i < PIECES; ++i) {
+            mbar_init(&d_full[i], 1);
+            mbar_init(&d_empty[i], SOFTMAX_WARPS + 3);
+        }
         mbar_init(unit_done, 2);
+        mbar_init(o_free, SOFTMAX_WARPS);
         *abort = 0;
         fence_mbar_init();
     }
@@ -264,60 +241,178 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
         tma_prefetch_desc(&vmap);
     }
     pdl_launch_dependents();
-    pdl_wait();  // lengths, queries and the cache come from the preceding kernels
-    if (warp == 0) find_share(p, share);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const Share sh = *share;
+    pdl_wait();  // lengths, queries and the cache come from the preceding kernels
     const uint32_t tmem = *tmem_addr;
 
-    if (warp == PRODUCER) {  // ------------------------------------------------- K and V tiles
-        regs_release<OTHER_REGS>();
-        const int rows_per_box = min(1 << p.s.page_shift, TILE);
+    // The next piece of the queue (all threads of a warp); rows 0 at its end
+    // or after an abort.
+    uint32_t taken = 0;
+    auto next_piece = [&](Piece &d) {
+        const uint32_t i = taken++;
+        const bool ok = warp_wait(&d_full[i % PIECES], (i / PIECES) & 1, abort, p.status);
+        d = queue[i % PIECES];
+        if (!ok) d.rows = 0;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&d_empty[i % PIECES]);
+        return d.rows > 0;
+    };
+
+    if (warp == SCHEDULER) {  // ------------------------------------------------- the CTA's pieces
+        int64_t total = 0, mine = 0;
+        for (int base = 0; base < p.s.seqs; base += 32) {
+            mine = 0;
+            if (base + lane < p.s.seqs) {
+                const SeqTiles q = seq_tiles(p, base + lane);
+                mine = q.tiles(p.s.kv_heads);
+                if (!q.sp.ok && blockIdx.x == 0) atomicExch(p.status, static_cast<unsigned>(DEV_BOUNDS));
+            }
+            int64_t sum = mine;
+#pragma unroll 1
+            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            total += sum;
+        }
+        if (total > 0x7FFFFFFF) {  // more cache than there can be
+            if (blockIdx.x == 0 && lane == 0) atomicExch(p.status, static_cast<unsigned>(DEV_BOUNDS));
+            total = 0;
+        }
+        Shares sh;
+        sh.grid = min(static_cast<int>(total), static_cast<int>(gridDim.x));
+        sh.per = sh.grid ? static_cast<int>(total) / sh.grid : 0;
+        sh.extra = static_cast<int>(total) - sh.per * sh.grid;
+        int pos = 0, end = 0, seq = 0, at = 0;
+        if (static_cast<int>(blockIdx.x) < sh.grid) {
+            pos = sh.begin(blockIdx.x);
+            end = sh.begin(blockIdx.x + 1);
+            int before = 0;
+            for (int base = 0; base < p.s.seqs; base += 32) {  // the sequence that holds tile `pos`
+                if (p.s.seqs > 32)
+                    mine = base + lane < p.s.seqs ? seq_tiles(p, base + lane).tiles(p.s.kv_heads) : 0;
+                int upto = static_cast<int>(mine);
+#pragma unroll 1
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += v;
+                }
+                const unsigned past = __ballot_sync(0xffffffffu, before + upto > pos);
+                if (past) {
+                    const int l = __ffs(past) - 1;
+                    seq = base + l;
+                    at = pos - before - __shfl_sync(0xffffffffu, upto - static_cast<int>(mine), l);
+                    break;
+                }
+                before += __shfl_sync(0xffffffffu, upto, 31);
+            }
+        }
+        SeqTiles q{};
+        int tiles = 0;
+        if (pos < end) q = seq_tiles(p, seq), tiles = static_cast<int>(q.tiles(p.s.kv_heads));
+        for (uint32_t i = 0;; ++i) {
+            Piece d{};
+            if (pos < end) {
+                while (at >= tiles) {
+                    at = 0;
+                    q = seq_tiles(p, ++seq);
+                    tiles = static_cast<int>(q.tiles(p.s.kv_heads));
+                }
+                const int unit = at / q.nt;
+                d.seq = seq;
+                d.first = q.sp.first;
+                d.n = q.n;
+                d.ctx = q.sp.ctx;
+                d.nt = q.nt;
+                d.t0 = at - unit * q.nt;
+                d.t1 = min(q.nt, d.t0 + end - pos);
+                d.kv = unit / q.units;
+                d.row0 = (unit - d.kv * q.units) * ROWS;
+                d.rows = min(ROWS, q.n * p.group - d.row0);
+                d.start = pos - d.t0;
+                d.owner0 = sh.owner(d.start);
+                d.ctas = sh.owner(d.start + d.nt - 1) - d.owner0 + 1;
+                pos += d.t1 - d.t0;
+                at += d.t1 - d.t0;
+            }
+            if (!warp_wait(&d_empty[i % PIECES], ((i / PIECES) & 1) ^ 1, abort, p.status)) break;
+            if (lane == 0) {
+                queue[i % PIECES] = d;
+                mbar_arrive(&d_full[i % PIECES]);
+            }
+            __syncwarp();
+            if (d.rows == 0) break;
+        }
+    } else if (warp == QUERIES) {  // ---------------------------------------------- query rows
+        QuerySlots slots;
+        Piece d;
+        while (next_piece(d)) {
+            const bool both = d.both();
+            const int slot = slots.take(both);
+            for (int s = slot; s <= (both ? 1 : slot); ++s) {
+                if (!warp_wait(&q_empty[s], slots.parity(s) ^ 1, abort, p.status)) break;
+                const int mask = (TILE >> d.copies()) - 1, row0 = both && s ? TILE : 0;
+                char *dst = qbuf + s * C::TILE_BYTES;
+                const uint16_t *src = p.a.q + static_cast<int64_t>(d.first) * p.a.ld_q +
+                                      static_cast<int64_t>(d.kv) * p.group * HD;
+#pragma unroll 4
+                for (int i = lane; i < TILE * (HD / 8); i += 32) {
+                    const int r = i / (HD / 8), c = i % (HD / 8), rr = row0 + (r & mask);
+                    const int x = d.row0 + (rr < d.rows ? rr : 0), node = x / p.group, g = x - node * p.group;
+                    copy16_async(dst + (c >> 3) * HALF_BYTES + r * 128 + (((c & 7) ^ (r & 7)) << 4),
+                                 src + node * p.a.ld_q + g * HD + c * 8, rr < d.rows);
+                }
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_full[s]);
+            }
+        }
+    } else if (warp == PRODUCER) {  // --------------------------------------------- K and V tiles
+        const int shift = p.s.page_shift, rows_per_box = min(1 << shift, TILE);
+        const int box = lane / C::HALVES, half = lane % C::HALVES;
         const uint64_t once = l2_evict_first(), again = l2_evict_normal();
         uint32_t seq_no = 0;  // ring position, over all pieces
-        bool live = true;
-        Walk walk(p, sh);
         Piece d;
-        while (live && walk.next(p, d)) {
+        while (next_piece(d)) {
             const int *table = p.t.page_table + d.seq * p.s.ld_table;
             // Several row tiles read the same cache: keep it in L2 for them.
             const uint64_t policy = d.n * p.group > ROWS ? again : once;
-            const int nt = d.t1 - d.t0;
-            for (int i = 0; i < 2 * nt && live; ++i, ++seq_no) {
-                // The order in which the MMA warp consumes them.
-                bool is_v;
-                int t;
-                if (d.both()) {
-                    is_v = i & 1;
-                    t = i >> 1;
-                } else {  // K0 K1 V0 K2 V1 .. K(nt-1) V(nt-2) V(nt-1)
-                    is_v = i == 2 * nt - 1 || (i >= 2 && !(i & 1));
-                    t = i == 2 * nt - 1 ? nt - 1 : is_v ? i / 2 - 1 : (i + 1) / 2;
-                }
-                const int pos = (d.t0 + t) * TILE;
-                const int valid = min(TILE, d.ctx + d.n - pos);
-                const int boxes = (valid + rows_per_box - 1) / rows_per_box * C::HALVES;
-                const int box = lane / C::HALVES, half = lane % C::HALVES;
-                int page = 0;
+            const int len = d.ctx + d.n;
+            // This lane's page of tile t; a page outside the pool becomes a
+            // coordinate outside the map, which reads zeros.
+            auto page_of = [&](int t) {
+                const int pos = t * TILE + box * rows_per_box;
+                return t < d.t1 && box < TILE / rows_per_box && pos < len ? table[pos >> shift] : 0;
+            };
+            auto load = [&](const CUtensorMap *map, int t, int page) {
+                const int pos = t * TILE, boxes = (min(TILE, len - pos) + rows_per_box - 1) / rows_per_box * C::HALVES;
+                const int stage = seq_no % C::STAGES;
+                if (!warp_wait(&empty[stage], ((seq_no / C::STAGES) & 1) ^ 1, abort, p.status)) return;  // never re-arm
+                if (lane == 0) mbar_arrive_expect_tx(&full[stage], boxes * rows_per_box * 128);
+                __syncwarp();
                 if (lane < boxes) {
-                    page = table[(pos + box * rows_per_box) >> p.s.page_shift];
-                    if (page < 0 || page >= p.s.pages) {  // a coordinate outside the map reads zeros
+                    if (page < 0 || page >= p.s.pages) {
                         atomicExch(p.status, static_cast<unsigned>(DEV_BOUNDS));
                         page = static_cast<int>(p.s.pages);
                     }
+                    tma_load_4d_hint(ring + stage * C::TILE_BYTES + half * HALF_BYTES + box * rows_per_box * 128, map,
+                                     &full[stage], half * 64, pos & ((1 << shift) - 1), d.kv, page, policy);
                 }
-                const int stage = seq_no % C::STAGES;
-                live = warp_wait(&empty[stage], ((seq_no / C::STAGES) & 1) ^ 1, abort, p.status);
-                if (!live) break;  // never re-arm after an abort
-                if (lane == 0) mbar_arrive_expect_tx(&full[stage], boxes * rows_per_box * 128);
                 __syncwarp();
-                if (lane < boxes)
-                    tma_load_4d_hint(ring + stage * C::TILE_BYTES + half * HALF_BYTES + box * rows_per_box * 128,
-                                     is_v ? &vmap : &kmap, &full[stage], half * 64, pos & ((1 << p.s.page_shift) - 1),
-                                     d.kv, page, policy);
-                __syncwarp();
+                ++seq_no;
+            };
+            // The order in which the MMA warp consumes them: with two row
+            // tiles K0 V0 K1 V1 .., else K0 K1 V0 K2 V1 .. (a tile's values
+            // follow the next tile's keys).
+            const int lag = d.both() ? 0 : 1;
+            int page = page_of(d.t0), page_v = page;
+#pragma unroll 1
+            for (int t = d.t0; t < d.t1 + lag && !*abort; ++t) {
+                const int ahead = page_of(t + 1);
+                if (t < d.t1) load(&kmap, t, page);
+                if (t - lag >= d.t0) load(&vmap, t - lag, lag ? page_v : page);
+                page_v = page;
+                page = ahead;
             }
         }
         // Copies in flight land before the CTA leaves.
@@ -325,23 +420,23 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
             const uint32_t i = seq_no - back;
             mbar_wait_drain(&full[i % C::STAGES], (i / C::STAGES) & 1);
         }
-    } else if (warp == MMA) {  // ------------------------------------------------ tensor cores
-        regs_release<OTHER_REGS>();
-        const uint32_t idesc_s = umma_idesc_bf16(128, TILE), idesc_o = umma_idesc_bf16(128, HD) | kUmmaTransposeB;
+    } else if (warp == MMA) {  // ---------------------------------------------------- tensor cores
+        // A negative scale negates the queries, so the running maximum can
+        // work on the scores as they come.
+        const uint32_t idesc_s = umma_idesc_bf16(128, TILE) | (p.a.scale < 0.0f ? kUmmaNegateA : 0u);
+        const uint32_t idesc_o = umma_idesc_bf16(128, HD) | kUmmaTransposeB;
         const uint32_t q_addr = smem_u32(qbuf), ring_addr = smem_u32(ring);
-        uint32_t base = 0, q_phase = 0, p_phase[2] = {0, 0};
+        uint32_t base = 0, p_phase = 0, pieces = 0;
         bool live = true;
-        Walk walk(p, sh);
+        QuerySlots slots;
         Piece d;
-        while (live && walk.next(p, d)) {
+        while (live && next_piece(d)) {
             const int nt = d.t1 - d.t0, items = d.items();
             const bool both = d.both();
-            live = warp_wait(q_full, q_phase, abort, p.status);
-            q_phase ^= 1;
+            const int slot = slots.take(both);
+            live = warp_wait(&q_full[slot], slots.parity(slot), abort, p.status);
+            if (live && both) live = warp_wait(&q_full[1], slots.parity(1), abort, p.status);
             if (!live) break;
-            tc_fence_after();
-            if (lane < 8) odd[lane] = 0u;
-            __syncwarp();
             auto scores = [&](int w) {
                 const int t = both ? w >> 1 : w, st = w & 1;
                 const uint32_t no = base + (both ? 2 * t : t == 0 ? 0 : 2 * t - 1);
@@ -349,7 +444,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                 if (!both || st == 0) live = warp_wait(&full[stage], (no / C::STAGES) & 1, abort, p.status);
                 if (!live) return;
                 if (lane == 0) {
-                    const uint32_t a = q_addr + (both ? st : 0) * C::TILE_BYTES, b = ring_addr + stage * C::TILE_BYTES;
+                    const uint32_t a = q_addr + (both ? st : slot) * C::TILE_BYTES, b = ring_addr + stage * C::TILE_BYTES;
 #pragma unroll
                     for (int ks = 0; ks < HD / 16; ++ks) {
                         const uint32_t off = (ks >> 2) * HALF_BYTES + (ks & 3) * 32;
@@ -365,11 +460,17 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                 const int t = both ? w >> 1 : w, st = w & 1;
                 const uint32_t no = base + (both ? 2 * t + 1 : t == nt - 1 ? 2 * nt - 1 : 2 * t + 2);
                 const int stage = no % C::STAGES;
+                if (w == 0) {  // the last piece's O and `odd` have been read
+                    if (pieces) live = warp_wait(o_free, (pieces - 1) & 1, abort, p.status);
+                    if (!live) return;
+                    if (lane < kMaxTreeNodes / 32) odd[lane] = 0u;
+                    __syncwarp();
+                }
                 if (!both || st == 0) {
                     live = warp_wait(&full[stage], (no / C::STAGES) & 1, abort, p.status);
                     if (!live) return;
                     const int pos = (d.t0 + t) * TILE, valid = min(TILE, d.ctx + d.n - pos);
-                    if (valid < TILE || pos + TILE > d.ctx) {
+                    if (pos + TILE > d.ctx) {
                         // A probability of zero does not hide what is not
                         // finite: rows behind the last position (never
                         // loaded, or whatever a page held) become zeros, and
@@ -378,35 +479,34 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                         // at the end.
                         char *v = ring + stage * C::TILE_BYTES;
                         const int from = max(0, d.ctx - pos);
-                        for (int i = from * 8 + lane; i < TILE * 8; i += 32) {
+#pragma unroll 4
+                        for (int i = from * (HD / 8) + lane; i < TILE * (HD / 8); i += 32) {
+                            const int row = i / (HD / 8), c = i % (HD / 8);
+                            uint4 *at = reinterpret_cast<uint4 *>(v + (c >> 3) * HALF_BYTES + row * 128 + (c & 7) * 16);
+                            if (row >= valid) {
+                                *at = make_uint4(0u, 0u, 0u, 0u);
+                                continue;
+                            }
+                            const uint4 u = *at;
+                            uint32_t x[4] = {u.x, u.y, u.z, u.w};
+                            bool bad = false;
 #pragma unroll
-                            for (int h = 0; h < C::HALVES; ++h) {
-                                uint4 *c = reinterpret_cast<uint4 *>(v + h * HALF_BYTES + i * 16);
-                                if ((i >> 3) >= valid) {
-                                    *c = make_uint4(0u, 0u, 0u, 0u);
-                                    continue;
-                                }
-                                const uint4 u = *c;
-                                uint32_t x[4] = {u.x, u.y, u.z, u.w};
-                                bool bad = false;
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    if ((x[e] & 0x7F80u) == 0x7F80u) x[e] &= 0xFFFF0000u, bad = true;
-                                    if ((x[e] & 0x7F800000u) == 0x7F800000u) x[e] &= 0x0000FFFFu, bad = true;
-                                }
-                                if (bad) {
-                                    *c = make_uint4(x[0], x[1], x[2], x[3]);
-                                    const int j = pos + (i >> 3) - d.ctx;
-                                    atomicOr(&odd[j >> 5], 1u << (j & 31));
-                                }
+                            for (int e = 0; e < 4; ++e) {
+                                if ((x[e] & 0x7F80u) == 0x7F80u) x[e] &= 0xFFFF0000u, bad = true;
+                                if ((x[e] & 0x7F800000u) == 0x7F800000u) x[e] &= 0x0000FFFFu, bad = true;
+                            }
+                            if (bad) {
+                                *at = make_uint4(x[0], x[1], x[2], x[3]);
+                                const int j = pos + row - d.ctx;
+                                atomicOr(&odd[j >> 5], 1u << (j & 31));
                             }
                         }
                         fence_proxy_async_smem();
                         __syncwarp();
                     }
                 }
-                live = warp_wait(&p_full[st], p_phase[st], abort, p.status);
-                p_phase[st] ^= 1;
+                live = warp_wait(&p_full[st], (p_phase >> st) & 1, abort, p.status);
+                p_phase ^= 1u << st;
                 if (!live) return;
                 tc_fence_after();
                 if (lane == 0) {
@@ -419,10 +519,9 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                 }
                 __syncwarp();
             };
-            scores(0);
-            if (live && items > 1) scores(1);
-            for (int w = 0; w < items && live; ++w) {
-                values(w);
+#pragma unroll 1
+            for (int w = -2; w < items && live; ++w) {
+                if (w >= 0) values(w);
                 if (live && w + 2 < items) scores(w + 2);
             }
             __syncwarp();
@@ -431,89 +530,73 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                 umma_commit(unit_done);
             }
             base += 2 * nt;
+            ++pieces;
         }
         // On the way out of an abort, MMAs in flight end before tensor memory is freed.
         if (!live) {
             if (lane == 0) umma_commit(&s_full[0]);
             for (int i = 0; i < 2; ++i) mbar_wait_drain(&s_full[0], i, 1000000ull);
         }
-    } else if (warp < SOFTMAX_WARPS) {  // ----------------------------------------- softmax
-        regs_claim<SOFTMAX_REGS>();
+    } else {  // ------------------------------------------------------------------------ softmax
         const int st = warp >> 2, r = tid & 127;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + lanes + st * TILE, to = tmem + lanes + 2 * TILE;
-        const float sc = (p.a.scale == 0.0f ? 1.0f : fabsf(p.a.scale)) * LOG2E;
+        const float sc = fabsf(p.a.scale) * LOG2E;
         uint32_t s_phase = 0, u_phase = 0;
-        bool head = false, tail = false;
-        Walk walk(p, sh);
+        bool shares[2] = {false, false};
+        QuerySlots slots;
         Piece d;
-        while (walk.next(p, d)) {
+        while (next_piece(d)) {
             const bool both = d.both();
-            // Queries, in the operand layout; zeros in rows that the unit lacks.
-            // A negative scale flips their signs and a zero one clears them,
-            // so the running maximum can work on the scores as they come.
-            const uint32_t flip = p.a.scale < 0.0f ? 0x80008000u : 0u;
-            const int chunks = (both ? ROWS : TILE) * (HD / 8);
-            for (int i = tid; i < chunks; i += 32 * SOFTMAX_WARPS) {
-                const int rr = i / (HD / 8), c = i % (HD / 8);
-                uint4 u = make_uint4(0u, 0u, 0u, 0u);
-                if (rr < d.rows && p.a.scale != 0.0f) {
-                    const int x = d.row0 + rr, node = x / p.group, g = x - node * p.group;
-                    u = *reinterpret_cast<const uint4 *>(p.a.q + (static_cast<int64_t>(d.first) + node) * p.a.ld_q +
-                                                         (static_cast<int64_t>(d.kv) * p.group + g) * HD + c * 8);
-                    u.x ^= flip, u.y ^= flip, u.z ^= flip, u.w ^= flip;
-                }
-                *reinterpret_cast<uint4 *>(qbuf + (rr >> 7) * C::TILE_BYTES + (c >> 3) * HALF_BYTES + (rr & 127) * 128 +
-                                           (((c & 7) ^ (rr & 7)) << 4)) = u;
-            }
-            fence_proxy_async_smem();
-            tc_fence_before();  // the last piece's reads of tensor memory, too
-            mbar_arrive(q_full);
-
-            const int rr = both ? st * TILE + r : r;  // this thread's row of the unit
+            const int slot = slots.take(both), copies = d.copies();
+            const int copy = r >> (7 - copies);             // which copy of the rows this thread holds
+            const int rr = both ? st * TILE + r : r & ((TILE >> copies) - 1);  // its row of the unit
             const bool mine = rr < d.rows;
             const bool warp_on = __any_sync(0xffffffffu, mine);
             const int x = d.row0 + rr, node = mine ? x / p.group : 0;
             const int64_t row = static_cast<int64_t>(d.first) + node;
             const RowMask mask{p.a.mask ? p.a.mask + row * p.s.mask_words : nullptr, d.n, node};
+            const int k0 = copy << (2 - copies), k1 = (copy + 1) << (2 - copies);  // its runs of 32 positions
             float m = -INFINITY, l = 0.0f;
             const int items = d.items();
+#pragma unroll 1
             for (int w = st; w < items; w += 2) {
                 mbar_wait(&s_full[st], s_phase, abort, p.status);
                 s_phase ^= 1;
                 tc_fence_after();
                 if (warp_on) {
-                    uint32_t v[4][32];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) tmem_ld_32x32b_x32(ts + 32 * k, v[k]);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) tie_regs(v[k]);
                     const int pos = (d.t0 + (both ? w >> 1 : w)) * TILE;
-                    if (pos + TILE > d.ctx) {
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
+                    uint32_t v[32];
+                    auto read = [&](int k) {  // 32 scores; hidden ones are -inf
+                        tmem_ld_32x32b_x32(ts + 32 * k, v);
+                        tmem_wait_ld();
+                        tie_regs(v);
+                        if (pos + 32 * k + 32 > d.ctx) {
                             const uint32_t see = mask.bits(pos + 32 * k - d.ctx);
 #pragma unroll
                             for (int e = 0; e < 32; ++e)
-                                if (!((see >> e) & 1u)) v[k][e] = 0xFF800000u;  // -inf
+                                if (!((see >> e) & 1u)) v[e] = 0xFF800000u;
                         }
-                    }
-                    float mx[4];
+                    };
+                    float top = -INFINITY;
+#pragma unroll 1
+                    for (int k = k1 - 1; k >= k0; --k) {
+                        read(k);
+                        float a = __uint_as_float(v[0]), b = __uint_as_float(v[1]);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        mx[k] = __uint_as_float(v[k][0]);
-#pragma unroll
-                        for (int e = 1; e < 32; ++e) mx[k] = fmaxf(mx[k], __uint_as_float(v[k][e]));
+                        for (int e = 2; e < 32; e += 2) {
+                            a = fmaxf(a, __uint_as_float(v[e]));
+                            b = fmaxf(b, __uint_as_float(v[e + 1]));
+                        }
+                        top = fmaxf(top, fmaxf(a, b));
                     }
-                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                     const bool raise = top > m && (m == -INFINITY || (top - m) * sc > RAISE);
                     if (__any_sync(0xffffffffu, raise)) {
                         const float corr = !raise ? 1.0f : m == -INFINITY ? 0.0f : exp2_approx((m - top) * sc);
                         if (raise) m = top;
                         l *= corr;
                         if (w >= 2) {  // this stream's O holds something
-#pragma unroll
+#pragma unroll 1
                             for (int c = 0; c < HD; c += 16) {
                                 uint32_t o[16];
                                 tmem_ld_32x32b_x16(to + st * HD + c, o);
@@ -526,18 +609,25 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                     }
                     const float off = m == -INFINITY ? 0.0f : m * sc;
                     float sum[2] = {0.0f, 0.0f};
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
+#pragma unroll 1
+                    for (int k = k0; k < k1; ++k) {
+                        if (k > k0) read(k);  // run k0 is in registers
                         uint32_t u[16];
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
-                            const float a = exp2_approx(fmaf(__uint_as_float(v[k][2 * e]), sc, -off));
-                            const float b = exp2_approx(fmaf(__uint_as_float(v[k][2 * e + 1]), sc, -off));
+                            const float a = exp2_approx(fmaf(__uint_as_float(v[2 * e]), sc, -off));
+                            const float b = exp2_approx(fmaf(__uint_as_float(v[2 * e + 1]), sc, -off));
                             u[e] = pack_bf16x2(a, b);
                             sum[0] += __uint_as_float(u[e] << 16);
                             sum[1] += __uint_as_float(u[e] & 0xFFFF0000u);
                         }
                         tmem_st_32x32b_x16(ts + 16 * k, u);
+                    }
+                    if (copies) {  // the other copies' positions
+                        const uint32_t zero[16] = {};
+#pragma unroll 1
+                        for (int k = 0; k < 4; ++k)
+                            if (k < k0 || k >= k1) tmem_st_32x32b_x16(ts + 16 * k, zero);
                     }
                     l += sum[0] + sum[1];
                     tmem_wait_st();
@@ -549,143 +639,204 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
             u_phase ^= 1;
             tc_fence_after();
 
-            // The piece's result: one stream's rows, or both streams' halves
-            // of the tiles joined (each warpgroup half of the dims).
-            // Log2 units; a row whose sum is NaN keeps a finite maximum, so
-            // that no join takes it for one that saw nothing.
+            // The piece's result.  Log2 units; a row whose sum is NaN keeps a
+            // finite maximum, so that no join takes it for one that saw nothing.
             const float m2 = l != l ? 0.0f : m == -INFINITY ? -INFINITY : m * sc;
-            float top = m2, lsum = l, w_own = m2 == -INFINITY ? 0.0f : 1.0f, w_other = 0.0f;
-            if (!both) {
-                float *ex = reinterpret_cast<float *>(qbuf);  // the queries are done with
-                ex[st * TILE + r] = m2;
-                ex[2 * TILE + st * TILE + r] = l;
-                named_bar_sync(1, 32 * SOFTMAX_WARPS);
-                const float mo = ex[(st ^ 1) * TILE + r], lo = ex[2 * TILE + (st ^ 1) * TILE + r];
-                named_bar_sync(1, 32 * SOFTMAX_WARPS);
-                top = fmaxf(m2, mo);
-                w_own = m2 == -INFINITY ? 0.0f : exp2_approx(m2 - top);
-                w_other = mo == -INFINITY ? 0.0f : exp2_approx(mo - top);
-                lsum = st == 0 ? l * w_own + lo * w_other : lo * w_other + l * w_own;
+            float top = m2, lsum = l, w0 = m2 == -INFINITY ? 0.0f : 1.0f, w1 = 0.0f;
+            char *scratch = qbuf + slot * C::TILE_BYTES;  // the queries are done with
+            if (!both) {  // join the streams' and copies' maxima and sums
+                float2 *ex = reinterpret_cast<float2 *>(scratch);
+                ex[st * TILE + r] = make_float2(m2, l);
+                named_bar_sync(1, SOFTMAX_THREADS);
+                top = -INFINITY;
+                const int states = 2 << copies, step = TILE >> copies;  // state i: stream i & 1, copy i >> 1
+#pragma unroll 1
+                for (int i = 0; i < states; ++i) top = fmaxf(top, ex[(i & 1) * TILE + (i >> 1) * step + rr].x);
+                lsum = 0.0f;
+#pragma unroll 1
+                for (int i = 0; i < states; ++i) {
+                    const float2 e = ex[(i & 1) * TILE + (i >> 1) * step + rr];
+                    const float wt = e.x == -INFINITY ? 0.0f : exp2_approx(e.x - top);
+                    lsum += e.y * wt;
+                    if (i >> 1 == copy) (i & 1 ? w1 : w0) = wt;
+                }
+                if (copies) named_bar_sync(1, SOFTMAX_THREADS);
             }
             const bool whole = d.t0 == 0 && d.t1 == d.nt;
-            float *rec = p.partial + (2 * static_cast<int64_t>(blockIdx.x) + (d.t0 == 0 ? 1 : 0)) * C::RECORD;
+            float *rec = p.partial + (2 * static_cast<int64_t>(blockIdx.x) + (d.t0 == 0 ? 1 : 0)) * C::RECORD + rr * HD;
+            uint16_t *out = p.a.out + row * p.a.ld_out +
+                            (static_cast<int64_t>(d.kv) * p.group + (x - node * p.group)) * HD;
+            // Each warpgroup takes all dims of its own rows, or half the dims of both streams' rows.
             const int dim0 = both ? 0 : st * (HD / 2), dim1 = both ? HD : dim0 + HD / 2;
-            const float w0 = both ? w_own : st == 0 ? w_own : w_other, w1 = both ? 0.0f : st == 0 ? w_other : w_own;
-            if (warp_on) {
-                for (int c = dim0; c < dim1; c += 32) {
-                    uint32_t a[32], b[32];
-                    float o[32];
-                    tmem_ld_32x32b_x32(to + (both ? st * HD : 0) + c, a);
-                    if (!both) tmem_ld_32x32b_x32(to + HD + c, b);
-                    tmem_wait_ld();
-                    tie_regs(a);
-                    if (!both) tie_regs(b);
+            const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
+            const bool any_odd = __any_sync(0xffffffffu, lane < kMaxTreeNodes / 32 && odd[lane & 7] != 0u);
+#pragma unroll 1
+            for (int phase = copies ? 0 : 1; phase < 2; ++phase) {
+                // Copies other than the first leave their rows in the scratch
+                // (phase 0) and the first adds them to its own.
+                if (warp_on && (copy == 0) == (phase == 1)) {
+#pragma unroll 1
+                    for (int c = dim0; c < dim1; c += 16) {
+                        uint32_t a[16], b[16];
+                        float o[16];
+                        tmem_ld_32x32b_x16(to + (both ? st * HD : 0) + c, a);
+                        if (!both) tmem_ld_32x32b_x16(to + HD + c, b);
+                        tmem_wait_ld(a);
+                        if (!both) tmem_wait_ld(b);
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        // a stream that saw nothing may hold anything
-                        o[e] = w0 == 0.0f ? 0.0f : __uint_as_float(a[e]) * w0;
-                        if (!both && w1 != 0.0f) o[e] = fmaf(__uint_as_float(b[e]), w1, o[e]);
-                    }
-                    // Infinities and NaN among the drafted values, for the rows that see them.
-                    for (int k = 0; k < 8; ++k) {
-                        uint32_t set = odd[k];
-                        if (set) set &= mask.word(k);
-                        for (; set && mine; set &= set - 1) {
-                            const int pos = d.ctx + 32 * k + __ffs(set) - 1;
-                            const int page = p.t.page_table[d.seq * p.s.ld_table + (pos >> p.s.page_shift)];
-                            if (page < 0 || page >= p.s.pages) continue;
-                            const uint16_t *src = p.a.v_cache + page * p.s.page_stride + d.kv * p.s.head_stride +
-                                                  (pos & ((1 << p.s.page_shift) - 1)) * p.s.token_stride + c;
+                        for (int e = 0; e < 16; ++e) {  // a stream that saw nothing may hold anything
+                            o[e] = w0 == 0.0f ? 0.0f : __uint_as_float(a[e]) * w0;
+                            if (!both && w1 != 0.0f) o[e] = fmaf(__uint_as_float(b[e]), w1, o[e]);
+                        }
+                        if (!mine) continue;
+                        if (phase == 0) {
+                            float4 *dst = reinterpret_cast<float4 *>(scratch) + ((copy - 1) * d.rows + rr) * (HD / 4) + c / 4;
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) {
-                                const uint16_t h = src[e];
-                                if ((h & 0x7F80u) == 0x7F80u) o[e] += bf16_bits_to_f32(h);
+                            for (int e = 0; e < 4; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                            continue;
+                        }
+#pragma unroll 1
+                        for (int i = 1; i < 1 << copies; ++i) {
+                            const float4 *src = reinterpret_cast<const float4 *>(scratch) + ((i - 1) * d.rows + rr) * (HD / 4) + c / 4;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float4 q = src[e];
+                                o[4 * e] += q.x, o[4 * e + 1] += q.y, o[4 * e + 2] += q.z, o[4 * e + 3] += q.w;
                             }
                         }
-                    }
-                    if (mine && whole) {
+                        if (whole) {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = finish(o[e], lsum);
-                        store_out(p.a.out + row * p.a.ld_out +
-                                      (static_cast<int64_t>(d.kv) * p.group + (x - node * p.group)) * HD + c,
-                                  o, p.a.out_pair_order);
-                    } else if (mine) {
+                            for (int e = 0; e < 16; ++e) o[e] *= inv;
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4)
-                            *reinterpret_cast<float4 *>(rec + rr * HD + c + e) =
-                                make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                            for (int e = 0; e < 16; e += 8) {
+                                auto pick = [&](int k) {
+                                    return p.a.out_pair_order ? pack_bf16x2(o[e + k], o[e + k + 4])
+                                                              : pack_bf16x2(o[e + 2 * k], o[e + 2 * k + 1]);
+                                };
+                                *reinterpret_cast<uint4 *>(out + c + e) = make_uint4(pick(0), pick(1), pick(2), pick(3));
+                            }
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 16; e += 4)
+                                *reinterpret_cast<float4 *>(rec + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                        }
                     }
+                    if (phase == 1 && any_odd && mine)
+                        add_odd_values(p, d, mask, odd, dim0, dim1, whole ? nullptr : rec, out);
                 }
-                if (mine && !whole && dim0 == 0) {
-                    rec[ROWS * HD + rr] = top;
-                    rec[ROWS * HD + ROWS + rr] = lsum;
-                }
+                if (phase == 0) named_bar_sync(1, SOFTMAX_THREADS);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(o_free);
+                mbar_arrive(&q_empty[slot]);
+                if (both) mbar_arrive(&q_empty[1]);
             }
             if (!whole) {
-                (d.t0 > 0 ? head : tail) = true;
-                if (tid == 0) shared_units[d.t0 > 0 ? 0 : 1] = d;
+                if (mine && copy == 0 && dim0 == 0) {
+                    float *ml = rec - rr * HD + ROWS * HD + rr;
+                    ml[0] = top;
+                    ml[ROWS] = lsum;
+                }
+                shares[d.t0 == 0] = true;
+                if (tid == 0) shared_units[d.t0 == 0] = d;
                 asm volatile("fence.acq_rel.gpu;" ::: "memory");
-                named_bar_sync(1, 32 * SOFTMAX_WARPS);
-                if (tid == 0) atomicAdd(&p.arrived[owner(sh, d.start)], 1u);
+                named_bar_sync(1, SOFTMAX_THREADS);
+                if (tid == 0) atomicAdd(&p.arrived[d.owner0], 1u);
             }
         }
-        // Merge the shared units: this CTA's share of their rows.
+        // Merge the shared units: this CTA's share of their rows.  A warp
+        // takes a row and a part of the unit's pieces.
+#pragma unroll 1
         for (int which = 0; which < 2; ++which) {
-            if (!(which ? tail : head)) continue;
+            if (!shares[which]) continue;
             const Piece u = shared_units[which];
-            const int c0 = owner(sh, u.start), c1 = owner(sh, u.start + u.nt - 1), k = c1 - c0 + 1;
-            const int me = blockIdx.x - c0;
+            const int k = u.ctas, me = blockIdx.x - u.owner0;
             const int r0 = u.rows * me / k, r1 = u.rows * (me + 1) / k;
             if (r1 > r0) {
-                if (tid == 0) {
+                bool ok = true;
+                if (lane == 0) {
                     const uint64_t since = globaltimer();
-                    int ok = 1;
-                    while (ok && *reinterpret_cast<volatile unsigned *>(&p.arrived[c0]) != static_cast<unsigned>(k)) {
+                    while (ok && *reinterpret_cast<volatile unsigned *>(&p.arrived[u.owner0]) != static_cast<unsigned>(k))
                         if (*abort || globaltimer() - since > kArrivalWaitNs) {
                             atomicExch(p.status, static_cast<unsigned>(DEV_TIMEOUT));
-                            ok = 0;
+                            ok = false;
+                        }
+                }
+                ok = __all_sync(0xffffffffu, ok);
+                asm volatile("fence.acq_rel.gpu;" ::: "memory");
+                constexpr int W = HD / 32;
+                // Warps of a row: as many as there are for the share's rows, each with at least two pieces.
+                int parts = 1;
+                while (2 * parts * (r1 - r0) <= SOFTMAX_WARPS && 4 * parts <= k) parts *= 2;
+                const int part = warp % parts;
+                float *ex = reinterpret_cast<float *>(ring);  // no copies are in flight any more
+#pragma unroll 1
+                for (int base = r0; base < r1; base += SOFTMAX_WARPS / parts) {
+                    const int rr = base + warp / parts;
+                    const bool on = ok && rr < r1;
+                    float top = -INFINITY, lsum = 0.0f, o[W];
+#pragma unroll
+                    for (int e = 0; e < W; ++e) o[e] = 0.0f;
+                    if (on) {
+                        const int j1 = k * (part + 1) / parts;
+#pragma unroll 1
+                        for (int j0 = k * part / parts; j0 < j1; j0 += 4) {
+                            float mj[4], lj[4], q[4][W];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {  // every load of four pieces first
+                                const int j = min(j0 + i, j1 - 1);
+                                const float *rec = p.partial + (2 * static_cast<int64_t>(u.owner0 + j) + (j == 0)) * C::RECORD;
+                                mj[i] = j0 + i < j1 ? __ldcg(rec + ROWS * HD + rr) : -INFINITY;
+                                lj[i] = __ldcg(rec + ROWS * HD + ROWS + rr);
+                                if (W == 4) *reinterpret_cast<float4 *>(q[i]) = __ldcg(reinterpret_cast<const float4 *>(rec + rr * HD) + lane);
+                                else *reinterpret_cast<float2 *>(q[i]) = __ldcg(reinterpret_cast<const float2 *>(rec + rr * HD) + lane);
+                            }
+                            const float t = fmaxf(fmaxf(fmaxf(mj[0], mj[1]), fmaxf(mj[2], mj[3])), top);
+                            const float keep = top == -INFINITY ? 0.0f : exp2_approx(top - t);
+                            top = t;
+                            lsum *= keep;
+#pragma unroll
+                            for (int e = 0; e < W; ++e) o[e] *= keep;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float wt = mj[i] == -INFINITY ? 0.0f : exp2_approx(mj[i] - t);
+                                if (wt != 0.0f) {
+                                    lsum = fmaf(lj[i], wt, lsum);
+#pragma unroll
+                                    for (int e = 0; e < W; ++e) o[e] = fmaf(q[i][e], wt, o[e]);
+                                }
+                            }
                         }
                     }
-                    *go = ok;
-                }
-                named_bar_sync(1, 32 * SOFTMAX_WARPS);
-                if (*go) {
-                    asm volatile("fence.acq_rel.gpu;" ::: "memory");
-                    constexpr int W = HD / 32;
-                    for (int rr = r0 + warp; rr < r1; rr += SOFTMAX_WARPS) {
-                        // weights: lanes over pieces
-                        float top = -INFINITY;
-                        for (int j = lane; j < k; j += 32)
-                            top = fmaxf(top, __ldcg(p.partial + (2 * static_cast<int64_t>(c0 + j) + (j == 0)) * C::RECORD +
-                                                    ROWS * HD + rr));
+                    if (parts > 1) {  // join the parts, in order, in the row's first warp
+                        float *my = ex + warp * (HD + 2);
+                        named_bar_sync(1, SOFTMAX_THREADS);
 #pragma unroll
-                        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                        float lsum = 0.0f, o[W];
+                        for (int e = 0; e < W; ++e) my[lane * W + e] = o[e];
+                        if (lane == 0) my[HD] = top, my[HD + 1] = lsum;
+                        named_bar_sync(1, SOFTMAX_THREADS);
+                        if (part == 0) {
+#pragma unroll 1
+                            for (int i = 1; i < parts; ++i) top = fmaxf(top, my[i * (HD + 2) + HD]);
+                            lsum = 0.0f;
 #pragma unroll
-                        for (int e = 0; e < W; ++e) o[e] = 0.0f;
-                        for (int j0 = 0; j0 < k; j0 += 32) {
-                            float wt = 0.0f;
-                            if (j0 + lane < k) {
-                                const float *rec = p.partial + (2 * static_cast<int64_t>(c0 + j0 + lane) + (j0 + lane == 0)) * C::RECORD;
-                                const float mj = __ldcg(rec + ROWS * HD + rr);
-                                wt = mj == -INFINITY ? 0.0f : exp2_approx(mj - top);
-                                lsum = fmaf(__ldcg(rec + ROWS * HD + ROWS + rr), wt, lsum);
-                            }
-                            const int cnt = min(32, k - j0);
-#pragma unroll 8
-                            for (int j = 0; j < cnt; ++j) {
-                                const float wj = __shfl_sync(0xffffffffu, wt, j);
-                                const float *rec = p.partial + (2 * static_cast<int64_t>(c0 + j0 + j) + (j0 + j == 0)) * C::RECORD +
-                                                   rr * HD + lane * W;
-                                float q[W];
-                                if (W == 4) *reinterpret_cast<float4 *>(q) = __ldcg(reinterpret_cast<const float4 *>(rec));
-                                else *reinterpret_cast<float2 *>(q) = __ldcg(reinterpret_cast<const float2 *>(rec));
+                            for (int e = 0; e < W; ++e) o[e] = 0.0f;
+#pragma unroll 1
+                            for (int i = 0; i < parts; ++i) {
+                                const float *q = my + i * (HD + 2);
+                                const float wt = q[HD] == -INFINITY ? 0.0f : exp2_approx(q[HD] - top);
+                                if (wt != 0.0f) {
+                                    lsum = fmaf(q[HD + 1], wt, lsum);
 #pragma unroll
-                                for (int e = 0; e < W; ++e) o[e] = fmaf(q[e], wj, o[e]);
+                                    for (int e = 0; e < W; ++e) o[e] = fmaf(q[lane * W + e], wt, o[e]);
+                                }
                             }
                         }
-#pragma unroll
-                        for (int s = 16; s; s >>= 1) lsum += __shfl_xor_sync(0xffffffffu, lsum, s);
+                    }
+                    if (on && part == 0) {
+                        const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
                         const int x = u.row0 + rr, node = x / p.group, g = x - node * p.group;
                         uint16_t *dst = p.a.out + (static_cast<int64_t>(u.first) + node) * p.a.ld_out +
                                         (static_cast<int64_t>(u.kv) * p.group + g) * HD;
@@ -693,20 +844,18 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                         for (int e = 0; e < W; ++e) {
                             const int dim = lane * W + e, in8 = dim & 7;
                             const int col = p.a.out_pair_order ? (dim & ~7) + (in8 < 4 ? 2 * in8 : 2 * (in8 - 4) + 1) : dim;
-                            dst[col] = f32_to_bf16_bits(finish(o[e], lsum));
+                            dst[col] = f32_to_bf16_bits(o[e] * inv);
                         }
                     }
                 }
-                named_bar_sync(1, 32 * SOFTMAX_WARPS);
             }
             // The last of the unit's CTAs clears its counters for the next launch.
-            if (tid == 0 && atomicAdd(&p.done[c0], 1u) == static_cast<unsigned>(k - 1)) {
-                atomicExch(&p.arrived[c0], 0u);
-                atomicExch(&p.done[c0], 0u);
+            named_bar_sync(1, SOFTMAX_THREADS);
+            if (tid == 0 && atomicAdd(&p.done[u.owner0], 1u) == static_cast<unsigned>(k - 1)) {
+                atomicExch(&p.arrived[u.owner0], 0u);
+                atomicExch(&p.done[u.owner0], 0u);
             }
         }
-    } else {
-        regs_release<OTHER_REGS>();
     }
     tc_fence_before();
     __syncthreads();

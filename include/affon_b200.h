@@ -418,7 +418,7 @@ int affon_b200_paged_append(affon_b200_ctx *ctx, const affon_b200_paged_desc *de
 typedef struct affon_b200_tree_attn_desc {
     uint32_t struct_size;
     int32_t q_heads;        /* a multiple of kv_heads */
-    float scale;
+    float scale;            /* finite, not zero */
     int32_t out_pair_order; /* write the output in 4-bit qmv pair order */
     int64_t ld_q, ld_out;
 } affon_b200_tree_attn_desc;
