@@ -106,14 +106,11 @@ struct Shares {
 // A piece of a unit: tiles [t0, t1) of nt.  rows 0 ends the queue.
 struct Piece {
     int seq, first, n, ctx, kv, row0, rows, t0, t1, nt;
-    int start;       // the unit's first tile in the order of all tiles
-    int owner0, ctas;  // the CTAs that share the unit
+    int start;  // the unit's first tile in the order of all tiles
     __device__ __forceinline__ bool both() const { return rows > TILE; }  // two row tiles, every position tile for both
     __device__ __forceinline__ int items() const { return both() ? 2 * (t1 - t0) : t1 - t0; }
-    // log2 of the copies of the rows in the 128 rows of the MMA: a copy's
-    // results are joined through the piece's own query buffer, which holds
-    // 64 + 64 rows of f32, or 3 x 16.
-    __device__ __forceinline__ int copies() const { return rows <= 16 ? 2 : rows <= 64 ? 1 : 0; }
+    // log2 of the copies of the rows in the 128 rows of the MMA.
+    __device__ __forceinline__ int copies() const { return rows <= 32 ? 2 : rows <= 64 ? 1 : 0; }
 };
 
 // Which of the two query buffers a piece uses and how often each was used.
@@ -149,15 +146,70 @@ struct RowMask {
     }
 };
 
-// A whole warp's wait, with one answer: false once any wait of the CTA gave up.
+// A whole warp's wait, with one answer: false when it gave up, or when another
+// wait of the CTA had.
 __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volatile int *abort, unsigned *status) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, status) && !*abort);
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, status));
 }
 
-// Copies 16 bytes to shared memory without registers (zeros when !take).
-__device__ __forceinline__ void copy16_async(void *dst, const void *src, bool take) {
-    const int bytes = take ? 16 : 0;
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
+// A value that is the same in all lanes, known as such to the compiler.
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+
+// Copies 16 bytes to shared memory without registers.
+__device__ __forceinline__ void copy16_async(void *dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+
+// 8 results of a row, dims in order or in the 4-bit qmv's pair order.
+__device__ __forceinline__ void store8_bf16(uint16_t *dst, const float (&o)[8], int pair_order) {
+    *reinterpret_cast<uint4 *>(dst) =
+        pair_order ? make_uint4(pack_bf16x2(o[0], o[4]), pack_bf16x2(o[1], o[5]), pack_bf16x2(o[2], o[6]),
+                                pack_bf16x2(o[3], o[7]))
+                   : make_uint4(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]), pack_bf16x2(o[4], o[5]),
+                                pack_bf16x2(o[6], o[7]));
+}
+// Output of row rr of a unit.
+template <int HD>
+__device__ __forceinline__ uint16_t *out_row(const Params &p, const Piece &d, int rr) {
+    const int x = d.row0 + rr, node = x / p.group, g = x - node * p.group;
+    return p.a.out + (static_cast<int64_t>(d.first) + node) * p.a.ld_out +
+           (static_cast<int64_t>(d.kv) * p.group + g) * HD;
+}
+template <int N>
+__device__ __forceinline__ void tmem_ld_row(uint32_t taddr, uint32_t (&r)[N]) {
+    if constexpr (N == 32) tmem_ld_32x32b_x32(taddr, r);
+    else tmem_ld_32x32b_x16(taddr, r);
+}
+template <int N>
+__device__ __forceinline__ void tie_row(uint32_t (&r)[N]) {
+    if constexpr (N == 32) tie_regs(r);
+    else tmem_wait_ld(r);
+}
+
+// Rows row0 .. row0+rows-1 of a unit into a query buffer (K-major, 128-byte
+// swizzle), 1 << copies times.  Rows that the unit lacks stay as they are: the
+// rows of the MMA do not mix.
+template <int HD>
+__device__ __forceinline__ void load_queries(const Params &p, const Piece &d, int row0, int rows, int copies, char *dst,
+                                             int thread, int threads) {
+    constexpr int CHUNKS = HD / 8;  // a thread keeps its 16 bytes of every step-th row
+    const int c = thread % CHUNKS, step = threads / CHUNKS, dn = step / p.group, dg = step - dn * p.group;
+    const int first = d.row0 + row0 + thread / CHUNKS;
+    int node = first / p.group, g = first - node * p.group;
+    const uint16_t *src = p.a.q + static_cast<int64_t>(d.first) * p.a.ld_q + static_cast<int64_t>(d.kv) * p.group * HD +
+                          c * 8;
+#pragma unroll 2
+    for (int r = thread / CHUNKS; r < rows; r += step) {
+        const uint16_t *from = src + node * p.a.ld_q + g * HD;
+        char *to = dst + (c >> 3) * HALF_BYTES + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+        copy16_async(to, from);
+        if (copies) copy16_async(to + TILE * 64, from);  // a copy's rows start at a multiple of 8
+        if (copies > 1) copy16_async(to + TILE * 32, from), copy16_async(to + TILE * 96, from);
+        g += dg, node += dn;
+        if (g >= p.group) g -= p.group, ++node;
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    fence_proxy_async_smem();
 }
 
 // Infinities and NaN among the drafted values, which were kept from the
@@ -187,6 +239,51 @@ __device__ __noinline__ void add_odd_values(const Params &p, const Piece &d, con
     }
 }
 
+// A probability of zero does not hide what is not finite.  Of a tile's drafted
+// positions (rows `from` to valid-1) the infinities and NaN, which only some
+// query rows see, become zeros and are noted; those rows get them back when
+// the piece ends.  Rows behind the last position that the last 16-position
+// step still takes (never loaded, or whatever a page held) become zeros.
+template <int HD>
+__device__ __forceinline__ void clean_values(char *v, int from, int valid, int node0, uint32_t *odd) {
+    constexpr int CHUNKS = HD / 8;
+    const int lane = threadIdx.x & 31;
+    auto at = [&](int i) {
+        return reinterpret_cast<uint4 *>(v + (i % CHUNKS >> 3) * HALF_BYTES + (i / CHUNKS) * 128 + (i & 7) * 16);
+    };
+    for (int i = valid * CHUNKS + lane; i < ((valid + 15) & ~15) * CHUNKS; i += 32) *at(i) = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll 1
+    for (int i0 = from * CHUNKS + lane; i0 < valid * CHUNKS; i0 += 128) {
+        uint4 u[4];
+        uint32_t bad[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) u[e] = i0 + 32 * e < valid * CHUNKS ? *at(i0 + 32 * e) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {  // an exponent of all ones carries into the sign's place
+            auto carry = [](uint32_t x) { return (x & 0x7F807F80u) + 0x00800080u; };
+            bad[e] = (carry(u[e].x) | carry(u[e].y) | carry(u[e].z) | carry(u[e].w)) & 0x80008000u;
+        }
+        if (!(bad[0] | bad[1] | bad[2] | bad[3])) continue;
+#pragma unroll 1
+        for (int e = 0; e < 4; ++e) {
+            const int i = i0 + 32 * e;
+            if (i >= valid * CHUNKS) break;
+            uint32_t *x = reinterpret_cast<uint32_t *>(at(i));
+            bool found = false;
+            for (int k = 0; k < 4; ++k) {
+                uint32_t y = x[k];
+                if ((y & 0x7F80u) == 0x7F80u) y &= 0xFFFF0000u, found = true;
+                if ((y & 0x7F800000u) == 0x7F800000u) y &= 0x0000FFFFu, found = true;
+                x[k] = y;
+            }
+            const int j = node0 + i / CHUNKS;
+            if (found) atomicOr(&odd[j >> 5], 1u << (j & 31));
+        }
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+}
+
 template <int HD>
 __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid_constant__ CUtensorMap kmap,
                                                                  const __grid_constant__ CUtensorMap vmap,
@@ -198,7 +295,8 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
     uint64_t *full = reinterpret_cast<uint64_t *>(ring + C::STAGES * C::TILE_BYTES);
     uint64_t *empty = full + C::STAGES;
     uint64_t *s_full = empty + C::STAGES;  // [2] scores of a stream are in tensor memory
-    uint64_t *p_full = s_full + 2;         // [2] probabilities of a stream are
+    uint64_t *p_half = s_full + 2;         // [2] probabilities of a tile's first 64 positions are
+    uint64_t *p_full = p_half + 2;         // [2] the rest
     uint64_t *q_full = p_full + 2;         // [2] query buffers
     uint64_t *q_empty = q_full + 2;
     uint64_t *d_full = q_empty + 2;        // [PIECES] the queue
@@ -207,11 +305,13 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
     uint64_t *o_free = unit_done + 1;        // its O has been read
     Piece *queue = reinterpret_cast<Piece *>(o_free + 1);
     Piece *shared_units = queue + PIECES;    // [2] pieces of shared units: the end of one, the start of another
-    uint32_t *odd = reinterpret_cast<uint32_t *>(shared_units + 2);  // drafted nodes whose values are not all finite
+    Shares *division = reinterpret_cast<Shares *>(shared_units + 2);
+    uint32_t *odd = reinterpret_cast<uint32_t *>(division + 1);  // drafted nodes whose values are not all finite
     uint32_t *tmem_addr = odd + kMaxTreeNodes / 32;
     volatile int *abort = reinterpret_cast<volatile int *>(tmem_addr + 1);
 
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // warp-uniform for the compiler, too
     if (tid == 0) {
         for (int i = 0; i < C::STAGES; ++i) {
             mbar_init(&full[i], 1);
@@ -219,6 +319,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
+            mbar_init(&p_half[i], 128);
             mbar_init(&p_full[i], 128);
             mbar_init(&q_full[i], 1);
             mbar_init(&q_empty[i], SOFTMAX_WARPS);
@@ -245,7 +346,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
     __syncthreads();
     tc_fence_after();
     pdl_wait();  // lengths, queries and the cache come from the preceding kernels
-    const uint32_t tmem = *tmem_addr;
+    const uint32_t tmem = static_cast<uint32_t>(uniform(static_cast<int>(*tmem_addr)));
 
     // The next piece of the queue (all threads of a warp); rows 0 at its end
     // or after an abort.
@@ -254,27 +355,28 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
         const uint32_t i = taken++;
         const bool ok = warp_wait(&d_full[i % PIECES], (i / PIECES) & 1, abort, p.status);
         d = queue[i % PIECES];
-        if (!ok) d.rows = 0;
+        d.rows = uniform(ok ? d.rows : 0);
         __syncwarp();
         if (lane == 0) mbar_arrive(&d_empty[i % PIECES]);
         return d.rows > 0;
     };
 
     if (warp == SCHEDULER) {  // ------------------------------------------------- the CTA's pieces
-        int64_t total = 0, mine = 0;
+        unsigned total = 0, mine = 0, high = 0;  // high: the total / 1024, should it not fit
         for (int base = 0; base < p.s.seqs; base += 32) {
             mine = 0;
+            unsigned part = 0;
             if (base + lane < p.s.seqs) {
                 const SeqTiles q = seq_tiles(p, base + lane);
-                mine = q.tiles(p.s.kv_heads);
+                const int64_t tiles = q.tiles(p.s.kv_heads);
+                mine = static_cast<unsigned>(tiles);
+                part = static_cast<unsigned>(min(tiles >> 10, int64_t(1) << 26));
                 if (!q.sp.ok && blockIdx.x == 0) atomicExch(p.status, static_cast<unsigned>(DEV_BOUNDS));
             }
-            int64_t sum = mine;
-#pragma unroll 1
-            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            total += sum;
+            total += __reduce_add_sync(0xffffffffu, mine);
+            high = min(high + __reduce_add_sync(0xffffffffu, part), 1u << 30);
         }
-        if (total > 0x7FFFFFFF) {  // more cache than there can be
+        if (high >= 1u << 20) {  // 2^30 tiles: more cache than there can be
             if (blockIdx.x == 0 && lane == 0) atomicExch(p.status, static_cast<unsigned>(DEV_BOUNDS));
             total = 0;
         }
@@ -289,7 +391,9 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
             int before = 0;
             for (int base = 0; base < p.s.seqs; base += 32) {  // the sequence that holds tile `pos`
                 if (p.s.seqs > 32)
-                    mine = base + lane < p.s.seqs ? seq_tiles(p, base + lane).tiles(p.s.kv_heads) : 0;
+                    mine = base + lane < p.s.seqs
+                               ? static_cast<unsigned>(seq_tiles(p, base + lane).tiles(p.s.kv_heads))
+                               : 0u;
                 int upto = static_cast<int>(mine);
 #pragma unroll 1
                 for (int o = 1; o < 32; o <<= 1) {
@@ -329,13 +433,12 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                 d.row0 = (unit - d.kv * q.units) * ROWS;
                 d.rows = min(ROWS, q.n * p.group - d.row0);
                 d.start = pos - d.t0;
-                d.owner0 = sh.owner(d.start);
-                d.ctas = sh.owner(d.start + d.nt - 1) - d.owner0 + 1;
                 pos += d.t1 - d.t0;
                 at += d.t1 - d.t0;
             }
             if (!warp_wait(&d_empty[i % PIECES], ((i / PIECES) & 1) ^ 1, abort, p.status)) break;
             if (lane == 0) {
+                if (i == 0) *division = sh;
                 queue[i % PIECES] = d;
                 mbar_arrive(&d_full[i % PIECES]);
             }
@@ -347,29 +450,18 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
         Piece d;
         while (next_piece(d)) {
             const bool both = d.both();
-            const int slot = slots.take(both);
-            for (int s = slot; s <= (both ? 1 : slot); ++s) {
-                if (!warp_wait(&q_empty[s], slots.parity(s) ^ 1, abort, p.status)) break;
-                const int mask = (TILE >> d.copies()) - 1, row0 = both && s ? TILE : 0;
-                char *dst = qbuf + s * C::TILE_BYTES;
-                const uint16_t *src = p.a.q + static_cast<int64_t>(d.first) * p.a.ld_q +
-                                      static_cast<int64_t>(d.kv) * p.group * HD;
-#pragma unroll 4
-                for (int i = lane; i < TILE * (HD / 8); i += 32) {
-                    const int r = i / (HD / 8), c = i % (HD / 8), rr = row0 + (r & mask);
-                    const int x = d.row0 + (rr < d.rows ? rr : 0), node = x / p.group, g = x - node * p.group;
-                    copy16_async(dst + (c >> 3) * HALF_BYTES + r * 128 + (((c & 7) ^ (r & 7)) << 4),
-                                 src + node * p.a.ld_q + g * HD + c * 8, rr < d.rows);
-                }
-                asm volatile("cp.async.wait_all;" ::: "memory");
-                fence_proxy_async_smem();
+            const int s = slots.take(both);
+            // Waits for every use in turn: a parity tells only neighbouring uses apart.
+            if (!warp_wait(&q_empty[s], slots.parity(s) ^ 1, abort, p.status)) break;
+            if (both && !warp_wait(&q_empty[1], slots.parity(1) ^ 1, abort, p.status)) break;
+            if (!both) {  // two row tiles are loaded by the softmax warps, who are free then
+                load_queries<HD>(p, d, 0, d.rows, d.copies(), qbuf + s * C::TILE_BYTES, lane, 32);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&q_full[s]);
             }
         }
     } else if (warp == PRODUCER) {  // --------------------------------------------- K and V tiles
         const int shift = p.s.page_shift, rows_per_box = min(1 << shift, TILE);
-        const int box = lane / C::HALVES, half = lane % C::HALVES;
         const uint64_t once = l2_evict_first(), again = l2_evict_normal();
         uint32_t seq_no = 0;  // ring position, over all pieces
         Piece d;
@@ -377,42 +469,50 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
             const int *table = p.t.page_table + d.seq * p.s.ld_table;
             // Several row tiles read the same cache: keep it in L2 for them.
             const uint64_t policy = d.n * p.group > ROWS ? again : once;
-            const int len = d.ctx + d.n;
-            // This lane's page of tile t; a page outside the pool becomes a
-            // coordinate outside the map, which reads zeros.
-            auto page_of = [&](int t) {
-                const int pos = t * TILE + box * rows_per_box;
-                return t < d.t1 && box < TILE / rows_per_box && pos < len ? table[pos >> shift] : 0;
-            };
-            auto load = [&](const CUtensorMap *map, int t, int page) {
-                const int pos = t * TILE, boxes = (min(TILE, len - pos) + rows_per_box - 1) / rows_per_box * C::HALVES;
+            const int t0 = uniform(d.t0), t1 = uniform(d.t1), len = uniform(d.ctx + d.n), kv = uniform(d.kv);
+            // The sequence's page table, 64 entries at a time, a lane two of
+            // them; the second half is fetched while the first is used.
+            const int last_page = (len - 1) >> shift;
+            int page0 = (t0 * TILE) >> shift;
+            auto fetch = [&](int i) { return table[min(i + lane, last_page)]; };
+            int ids = fetch(page0), more = fetch(page0 + 32);
+            auto load = [&](const CUtensorMap *map, int t) {
+                const int pos = t * TILE, boxes = (min(TILE, len - pos) + rows_per_box - 1) / rows_per_box;
                 const int stage = seq_no % C::STAGES;
-                if (!warp_wait(&empty[stage], ((seq_no / C::STAGES) & 1) ^ 1, abort, p.status)) return;  // never re-arm
-                if (lane == 0) mbar_arrive_expect_tx(&full[stage], boxes * rows_per_box * 128);
+                if (!warp_wait(&empty[stage], ((seq_no / C::STAGES) & 1) ^ 1, abort, p.status) ||
+                    __any_sync(0xffffffffu, *abort))
+                    return;  // never re-arm a stage after an abort
+                if (lane == 0) mbar_arrive_expect_tx(&full[stage], boxes * C::HALVES * rows_per_box * 128);
                 __syncwarp();
-                if (lane < boxes) {
-                    if (page < 0 || page >= p.s.pages) {
-                        atomicExch(p.status, static_cast<unsigned>(DEV_BOUNDS));
+                char *dst = ring + stage * C::TILE_BYTES;
+#pragma unroll 1
+                for (int b = 0; b < boxes; ++b) {
+                    const int i = ((pos + b * rows_per_box) >> shift) - page0;
+                    int page = uniform(__shfl_sync(0xffffffffu, i < 32 ? ids : more, i & 31));
+                    if (page < 0 || page >= p.s.pages) {  // a coordinate outside the map reads zeros
+                        if (lane == 0) atomicExch(p.status, static_cast<unsigned>(DEV_BOUNDS));
                         page = static_cast<int>(p.s.pages);
                     }
-                    tma_load_4d_hint(ring + stage * C::TILE_BYTES + half * HALF_BYTES + box * rows_per_box * 128, map,
-                                     &full[stage], half * 64, pos & ((1 << shift) - 1), d.kv, page, policy);
+#pragma unroll
+                    for (int h = 0; h < C::HALVES; ++h)
+                        tma_load_4d_elect(dst + h * HALF_BYTES + b * rows_per_box * 128, map, &full[stage], h * 64,
+                                          pos & ((1 << shift) - 1), kv, page, policy);
                 }
-                __syncwarp();
                 ++seq_no;
             };
             // The order in which the MMA warp consumes them: with two row
             // tiles K0 V0 K1 V1 .., else K0 K1 V0 K2 V1 .. (a tile's values
             // follow the next tile's keys).
-            const int lag = d.both() ? 0 : 1;
-            int page = page_of(d.t0), page_v = page;
+            const int lag = uniform(d.both() ? 0 : 1);
 #pragma unroll 1
-            for (int t = d.t0; t < d.t1 + lag && !*abort; ++t) {
-                const int ahead = page_of(t + 1);
-                if (t < d.t1) load(&kmap, t, page);
-                if (t - lag >= d.t0) load(&vmap, t - lag, lag ? page_v : page);
-                page_v = page;
-                page = ahead;
+            for (int t = t0; t < t1 + lag && !*abort; ++t) {
+                if (((t - lag) * TILE >> shift) - page0 >= 32 && t > t0) {  // the first half is used up
+                    page0 += 32;
+                    ids = more;
+                    more = fetch(page0 + 32);
+                }
+                if (t < t1) load(&kmap, t);
+                if (t - lag >= t0) load(&vmap, t - lag);
             }
         }
         // Copies in flight land before the CTA leaves.
@@ -431,9 +531,10 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
         QuerySlots slots;
         Piece d;
         while (live && next_piece(d)) {
-            const int nt = d.t1 - d.t0, items = d.items();
-            const bool both = d.both();
-            const int slot = slots.take(both);
+            const int nt = uniform(d.t1 - d.t0), both = uniform(d.both()), items = both ? 2 * nt : nt;
+            const bool halves = uniform(d.copies() == 0);  // P comes in two halves
+            const int tile0 = uniform(d.t0), ctx = uniform(d.ctx), len = uniform(d.ctx + d.n);
+            const int slot = uniform(slots.take(both));
             live = warp_wait(&q_full[slot], slots.parity(slot), abort, p.status);
             if (live && both) live = warp_wait(&q_full[1], slots.parity(1), abort, p.status);
             if (!live) break;
@@ -443,18 +544,15 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                 const int stage = no % C::STAGES;
                 if (!both || st == 0) live = warp_wait(&full[stage], (no / C::STAGES) & 1, abort, p.status);
                 if (!live) return;
-                if (lane == 0) {
-                    const uint32_t a = q_addr + (both ? st : slot) * C::TILE_BYTES, b = ring_addr + stage * C::TILE_BYTES;
+                const uint64_t a = umma_desc_sw128(q_addr + (both ? st : slot) * C::TILE_BYTES);
+                const uint64_t b = umma_desc_sw128(ring_addr + stage * C::TILE_BYTES);
 #pragma unroll
-                    for (int ks = 0; ks < HD / 16; ++ks) {
-                        const uint32_t off = (ks >> 2) * HALF_BYTES + (ks & 3) * 32;
-                        umma_bf16_ss(tmem + st * TILE, umma_desc_sw128(a + off), umma_desc_sw128(b + off), idesc_s,
-                                     ks > 0);
-                    }
-                    umma_commit(&s_full[st]);
-                    if (!both || st == 1) umma_commit(&empty[stage]);
+                for (int ks = 0; ks < HD / 16; ++ks) {  // the descriptors' addresses count 16 bytes
+                    const uint32_t off = ((ks >> 2) * HALF_BYTES + (ks & 3) * 32) >> 4;
+                    umma_bf16_ss_elect(tmem + st * TILE, a + off, b + off, idesc_s, ks > 0);
                 }
-                __syncwarp();
+                umma_commit_elect(&s_full[st]);
+                if (!both || st == 1) umma_commit_elect(&empty[stage]);
             };
             auto values = [&](int w) {
                 const int t = both ? w >> 1 : w, st = w & 1;
@@ -466,58 +564,40 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                     if (lane < kMaxTreeNodes / 32) odd[lane] = 0u;
                     __syncwarp();
                 }
+                const int pos = (tile0 + t) * TILE, valid = min(TILE, len - pos);
                 if (!both || st == 0) {
                     live = warp_wait(&full[stage], (no / C::STAGES) & 1, abort, p.status);
                     if (!live) return;
-                    const int pos = (d.t0 + t) * TILE, valid = min(TILE, d.ctx + d.n - pos);
-                    if (pos + TILE > d.ctx) {
-                        // A probability of zero does not hide what is not
-                        // finite: rows behind the last position (never
-                        // loaded, or whatever a page held) become zeros, and
-                        // so do the infinities and NaN of drafted values,
-                        // which only some rows see; those rows get them back
-                        // at the end.
-                        char *v = ring + stage * C::TILE_BYTES;
-                        const int from = max(0, d.ctx - pos);
-#pragma unroll 4
-                        for (int i = from * (HD / 8) + lane; i < TILE * (HD / 8); i += 32) {
-                            const int row = i / (HD / 8), c = i % (HD / 8);
-                            uint4 *at = reinterpret_cast<uint4 *>(v + (c >> 3) * HALF_BYTES + row * 128 + (c & 7) * 16);
-                            if (row >= valid) {
-                                *at = make_uint4(0u, 0u, 0u, 0u);
-                                continue;
-                            }
-                            const uint4 u = *at;
-                            uint32_t x[4] = {u.x, u.y, u.z, u.w};
-                            bool bad = false;
+                    if (pos + TILE > ctx)
+                        clean_values<HD>(ring + stage * C::TILE_BYTES, max(0, ctx - pos), valid, pos - ctx, odd);
+                }
+                // 16 positions a step; steps behind the last position are left out.
+                const int steps = (valid + 15) >> 4;
+                const uint64_t b = umma_desc_mn_sw128(ring_addr + stage * C::TILE_BYTES, HALF_BYTES);
+                auto product = [&](int ks) {
+                    if (ks < steps)
+                        umma_bf16_ts_elect(tmem + 2 * TILE + st * HD, tmem + st * TILE + ks * 8, b + ks * (2048 >> 4),
+                                           idesc_o, w >= 2 || ks > 0);
+                };
+                if (halves) {
+                    live = warp_wait(&p_half[st], (p_phase >> (2 + st)) & 1, abort, p.status);
+                    p_phase ^= 4u << st;
+                    if (!live) return;
+                    tc_fence_after();
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                if ((x[e] & 0x7F80u) == 0x7F80u) x[e] &= 0xFFFF0000u, bad = true;
-                                if ((x[e] & 0x7F800000u) == 0x7F800000u) x[e] &= 0x0000FFFFu, bad = true;
-                            }
-                            if (bad) {
-                                *at = make_uint4(x[0], x[1], x[2], x[3]);
-                                const int j = pos + row - d.ctx;
-                                atomicOr(&odd[j >> 5], 1u << (j & 31));
-                            }
-                        }
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                    }
+                    for (int ks = 0; ks < 4; ++ks) product(ks);
                 }
                 live = warp_wait(&p_full[st], (p_phase >> st) & 1, abort, p.status);
                 p_phase ^= 1u << st;
                 if (!live) return;
                 tc_fence_after();
-                if (lane == 0) {
-                    const uint32_t b = ring_addr + stage * C::TILE_BYTES;
+                if (!halves) {
 #pragma unroll
-                    for (int ks = 0; ks < TILE / 16; ++ks)
-                        umma_bf16_ts(tmem + 2 * TILE + st * HD, tmem + st * TILE + ks * 8,
-                                     umma_desc_mn_sw128(b + ks * 2048, HALF_BYTES), idesc_o, w >= 2 || ks > 0);
-                    if (!both || st == 1) umma_commit(&empty[stage]);
+                    for (int ks = 0; ks < 4; ++ks) product(ks);
                 }
-                __syncwarp();
+#pragma unroll
+                for (int ks = 4; ks < TILE / 16; ++ks) product(ks);
+                if (!both || st == 1) umma_commit_elect(&empty[stage]);
             };
 #pragma unroll 1
             for (int w = -2; w < items && live; ++w) {
@@ -525,16 +605,14 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                 if (live && w + 2 < items) scores(w + 2);
             }
             __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(unit_done);  // `odd` is written
-                umma_commit(unit_done);
-            }
+            if (lane == 0) mbar_arrive(unit_done);  // `odd` is written
+            umma_commit_elect(unit_done);
             base += 2 * nt;
             ++pieces;
         }
         // On the way out of an abort, MMAs in flight end before tensor memory is freed.
         if (!live) {
-            if (lane == 0) umma_commit(&s_full[0]);
+            umma_commit_elect(&s_full[0]);
             for (int i = 0; i < 2; ++i) mbar_wait_drain(&s_full[0], i, 1000000ull);
         }
     } else {  // ------------------------------------------------------------------------ softmax
@@ -556,6 +634,12 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
             const int x = d.row0 + rr, node = mine ? x / p.group : 0;
             const int64_t row = static_cast<int64_t>(d.first) + node;
             const RowMask mask{p.a.mask ? p.a.mask + row * p.s.mask_words : nullptr, d.n, node};
+            if (both) {
+                mbar_wait(&q_empty[st], slots.parity(st) ^ 1, abort, p.status);
+                load_queries<HD>(p, d, st * TILE, min(TILE, d.rows - st * TILE), 0, qbuf + st * C::TILE_BYTES, r, 128);
+                named_bar_sync(2 + st, 128);
+                if (r == 0) mbar_arrive(&q_full[st]);
+            }
             const int k0 = copy << (2 - copies), k1 = (copy + 1) << (2 - copies);  // its runs of 32 positions
             float m = -INFINITY, l = 0.0f;
             const int items = d.items();
@@ -566,31 +650,51 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                 tc_fence_after();
                 if (warp_on) {
                     const int pos = (d.t0 + (both ? w >> 1 : w)) * TILE;
-                    uint32_t v[32];
-                    auto read = [&](int k) {  // 32 scores; hidden ones are -inf
-                        tmem_ld_32x32b_x32(ts + 32 * k, v);
+                    if (pos + TILE > d.ctx) {  // drafted positions, or the end: hidden scores become -inf
+#pragma unroll 1
+                        for (int k = 2 * k0; k < 2 * k1; ++k) {
+                            uint32_t x[16];
+                            tmem_ld_32x32b_x16(ts + 16 * k, x);
+                            const uint32_t see = mask.bits(pos + 16 * k - d.ctx);
+                            tmem_wait_ld(x);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e)
+                                if (!((see >> e) & 1u)) x[e] = 0xFF800000u;
+                            tmem_st_32x32b_x16(ts + 16 * k, x);
+                        }
+                        tmem_wait_st();
+                    }
+                    // Runs of 32 positions, the next one on its way while one
+                    // is worked on.
+                    uint32_t v0[32], v1[32];
+                    auto arrive = [&](uint32_t (&v)[32]) {
                         tmem_wait_ld();
                         tie_regs(v);
-                        if (pos + 32 * k + 32 > d.ctx) {
-                            const uint32_t see = mask.bits(pos + 32 * k - d.ctx);
-#pragma unroll
-                            for (int e = 0; e < 32; ++e)
-                                if (!((see >> e) & 1u)) v[e] = 0xFF800000u;
-                        }
                     };
                     float top = -INFINITY;
-#pragma unroll 1
-                    for (int k = k1 - 1; k >= k0; --k) {
-                        read(k);
-                        float a = __uint_as_float(v[0]), b = __uint_as_float(v[1]);
+                    auto raise_top = [&](const uint32_t (&v)[32]) {
+                        float a[4];
 #pragma unroll
-                        for (int e = 2; e < 32; e += 2) {
-                            a = fmaxf(a, __uint_as_float(v[e]));
-                            b = fmaxf(b, __uint_as_float(v[e + 1]));
+                        for (int e = 0; e < 4; ++e) a[e] = __uint_as_float(v[e]);
+#pragma unroll
+                        for (int e = 4; e < 32; ++e) a[e & 3] = fmaxf(a[e & 3], __uint_as_float(v[e]));
+                        top = fmaxf(top, fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])));
+                    };
+                    const bool single = k1 - k0 == 1;
+                    if (single) tmem_ld_32x32b_x32(ts + 32 * k0, v1);
+                    else tmem_ld_32x32b_x32(ts + 32 * (k1 - 1), v0);
+#pragma unroll 1
+                    for (int k = k1 - 1; k >= k0; k -= 2) {  // downwards: run k0 ends up in v1
+                        if (!single) {
+                            arrive(v0);
+                            tmem_ld_32x32b_x32(ts + 32 * (k - 1), v1);
+                            raise_top(v0);
                         }
-                        top = fmaxf(top, fmaxf(a, b));
+                        arrive(v1);
+                        if (k - 2 >= k0) tmem_ld_32x32b_x32(ts + 32 * (k - 2), v0);
+                        raise_top(v1);
                     }
-                    const bool raise = top > m && (m == -INFINITY || (top - m) * sc > RAISE);
+                    const bool raise = mine && top > m && (m == -INFINITY || (top - m) * sc > RAISE);
                     if (__any_sync(0xffffffffu, raise)) {
                         const float corr = !raise ? 1.0f : m == -INFINITY ? 0.0f : exp2_approx((m - top) * sc);
                         if (raise) m = top;
@@ -609,19 +713,33 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                     }
                     const float off = m == -INFINITY ? 0.0f : m * sc;
                     float sum[2] = {0.0f, 0.0f};
-#pragma unroll 1
-                    for (int k = k0; k < k1; ++k) {
-                        if (k > k0) read(k);  // run k0 is in registers
+                    auto weigh = [&](const uint32_t (&x)[32], int run) {
                         uint32_t u[16];
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
-                            const float a = exp2_approx(fmaf(__uint_as_float(v[2 * e]), sc, -off));
-                            const float b = exp2_approx(fmaf(__uint_as_float(v[2 * e + 1]), sc, -off));
+                            const float a = exp2_approx(fmaf(__uint_as_float(x[2 * e]), sc, -off));
+                            const float b = exp2_approx(fmaf(__uint_as_float(x[2 * e + 1]), sc, -off));
                             u[e] = pack_bf16x2(a, b);
                             sum[0] += __uint_as_float(u[e] << 16);
                             sum[1] += __uint_as_float(u[e] & 0xFFFF0000u);
                         }
-                        tmem_st_32x32b_x16(ts + 16 * k, u);
+                        tmem_st_32x32b_x16(ts + 16 * run, u);  // over scores that have been read
+                    };
+#pragma unroll 1
+                    for (int k = k0; k < k1; k += 2) {
+                        if (!single) tmem_ld_32x32b_x32(ts + 32 * (k + 1), v0);
+                        weigh(v1, k);
+                        if (!single) {
+                            arrive(v0);
+                            if (k + 2 < k1) tmem_ld_32x32b_x32(ts + 32 * (k + 2), v1);
+                            weigh(v0, k + 1);
+                            if (k + 2 < k1) {
+                                tmem_wait_st();  // the first half of the row's probabilities
+                                tc_fence_before();
+                                mbar_arrive(&p_half[st]);
+                                arrive(v1);
+                            }
+                        }
                     }
                     if (copies) {  // the other copies' positions
                         const uint32_t zero[16] = {};
@@ -633,6 +751,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                     tmem_wait_st();
                 }
                 tc_fence_before();
+                if (!copies && !warp_on) mbar_arrive(&p_half[st]);
                 mbar_arrive(&p_full[st]);
             }
             mbar_wait(unit_done, u_phase, abort, p.status);
@@ -648,83 +767,89 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                 float2 *ex = reinterpret_cast<float2 *>(scratch);
                 ex[st * TILE + r] = make_float2(m2, l);
                 named_bar_sync(1, SOFTMAX_THREADS);
-                top = -INFINITY;
                 const int states = 2 << copies, step = TILE >> copies;  // state i: stream i & 1, copy i >> 1
-#pragma unroll 1
-                for (int i = 0; i < states; ++i) top = fmaxf(top, ex[(i & 1) * TILE + (i >> 1) * step + rr].x);
+                float2 e[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    e[i] = i < states ? ex[(i & 1) * TILE + (i >> 1) * step + rr] : make_float2(-INFINITY, 0.0f);
+                top = -INFINITY;
                 lsum = 0.0f;
-#pragma unroll 1
-                for (int i = 0; i < states; ++i) {
-                    const float2 e = ex[(i & 1) * TILE + (i >> 1) * step + rr];
-                    const float wt = e.x == -INFINITY ? 0.0f : exp2_approx(e.x - top);
-                    lsum += e.y * wt;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top = fmaxf(top, e[i].x);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float wt = e[i].x == -INFINITY ? 0.0f : exp2_approx(e[i].x - top);
+                    lsum += e[i].y * wt;
                     if (i >> 1 == copy) (i & 1 ? w1 : w0) = wt;
                 }
-                if (copies) named_bar_sync(1, SOFTMAX_THREADS);
+                named_bar_sync(1, SOFTMAX_THREADS);
             }
             const bool whole = d.t0 == 0 && d.t1 == d.nt;
-            float *rec = p.partial + (2 * static_cast<int64_t>(blockIdx.x) + (d.t0 == 0 ? 1 : 0)) * C::RECORD + rr * HD;
-            uint16_t *out = p.a.out + row * p.a.ld_out +
-                            (static_cast<int64_t>(d.kv) * p.group + (x - node * p.group)) * HD;
-            // Each warpgroup takes all dims of its own rows, or half the dims of both streams' rows.
+            if (whole) {
+                const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
+                w0 *= inv, w1 *= inv;
+            }
+            // O in rounds of HD/4 dims: a thread leaves its row's in shared
+            // memory, then the warpgroup adds the copies up and stores whole
+            // sectors.  Each warpgroup takes all dims of its own rows, or
+            // half the dims of both streams' rows.
+            constexpr int W = HD / 4, CH = W / 8;
             const int dim0 = both ? 0 : st * (HD / 2), dim1 = both ? HD : dim0 + HD / 2;
-            const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
-            const bool any_odd = __any_sync(0xffffffffu, lane < kMaxTreeNodes / 32 && odd[lane & 7] != 0u);
+            const int rows = both ? min(TILE, d.rows - st * TILE) : d.rows;
+            const bool pair = !both && items > 1;  // the second stream's O holds something
+            char *stage = both ? qbuf + st * C::TILE_BYTES : scratch + st * (C::TILE_BYTES / 2);
+            auto cell = [&](int row, int c) {  // 16 bytes, spread over the banks
+                return reinterpret_cast<float4 *>(stage + row * (W * 4) + ((c ^ (row >> (HD == 64) & (W / 4 - 1))) << 4));
+            };
+            float *rec = p.partial + (2 * static_cast<int64_t>(blockIdx.x) + (d.t0 == 0 ? 1 : 0)) * C::RECORD;
+            const int lead = both ? st * TILE : 0;
 #pragma unroll 1
-            for (int phase = copies ? 0 : 1; phase < 2; ++phase) {
-                // Copies other than the first leave their rows in the scratch
-                // (phase 0) and the first adds them to its own.
-                if (warp_on && (copy == 0) == (phase == 1)) {
-#pragma unroll 1
-                    for (int c = dim0; c < dim1; c += 16) {
-                        uint32_t a[16], b[16];
-                        float o[16];
-                        tmem_ld_32x32b_x16(to + (both ? st * HD : 0) + c, a);
-                        if (!both) tmem_ld_32x32b_x16(to + HD + c, b);
-                        tmem_wait_ld(a);
-                        if (!both) tmem_wait_ld(b);
+            for (int c = dim0; c < dim1; c += W) {
+                if (warp_on) {
+                    uint32_t a[W], b[W];
+                    tmem_ld_row<W>(to + (both ? st * HD : 0) + c, a);
+                    if (pair) tmem_ld_row<W>(to + HD + c, b);
+                    tmem_wait_ld();
+                    tie_row<W>(a);
+                    tie_row<W>(b);
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) {  // a stream that saw nothing may hold anything
-                            o[e] = w0 == 0.0f ? 0.0f : __uint_as_float(a[e]) * w0;
-                            if (!both && w1 != 0.0f) o[e] = fmaf(__uint_as_float(b[e]), w1, o[e]);
+                    for (int e = 0; e < W; e += 4) {
+                        float o[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            o[i] = __uint_as_float(a[e + i]) * w0;
+                            if (pair) o[i] = fmaf(__uint_as_float(b[e + i]), w1, o[i]);
                         }
-                        if (!mine) continue;
-                        if (phase == 0) {
-                            float4 *dst = reinterpret_cast<float4 *>(scratch) + ((copy - 1) * d.rows + rr) * (HD / 4) + c / 4;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-                            continue;
-                        }
-#pragma unroll 1
-                        for (int i = 1; i < 1 << copies; ++i) {
-                            const float4 *src = reinterpret_cast<const float4 *>(scratch) + ((i - 1) * d.rows + rr) * (HD / 4) + c / 4;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const float4 q = src[e];
-                                o[4 * e] += q.x, o[4 * e + 1] += q.y, o[4 * e + 2] += q.z, o[4 * e + 3] += q.w;
-                            }
-                        }
-                        if (whole) {
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) o[e] *= inv;
-#pragma unroll
-                            for (int e = 0; e < 16; e += 8) {
-                                auto pick = [&](int k) {
-                                    return p.a.out_pair_order ? pack_bf16x2(o[e + k], o[e + k + 4])
-                                                              : pack_bf16x2(o[e + 2 * k], o[e + 2 * k + 1]);
-                                };
-                                *reinterpret_cast<uint4 *>(out + c + e) = make_uint4(pick(0), pick(1), pick(2), pick(3));
-                            }
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 16; e += 4)
-                                *reinterpret_cast<float4 *>(rec + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-                        }
+                        if (mine) *cell(r, e / 4) = make_float4(o[0], o[1], o[2], o[3]);
                     }
-                    if (phase == 1 && any_odd && mine)
-                        add_odd_values(p, d, mask, odd, dim0, dim1, whole ? nullptr : rec, out);
                 }
-                if (phase == 0) named_bar_sync(1, SOFTMAX_THREADS);
+                named_bar_sync(2 + st, 128);
+#pragma unroll 1
+                for (int i = r; i < rows * CH; i += 128) {
+                    const int row = i / CH, k = i % CH;  // 8 dims of a row
+                    float o[8] = {};
+#pragma unroll 1
+                    for (int q = 0; q < 1 << copies; ++q) {
+                        const float4 x0 = *cell(row + q * (TILE >> copies), 2 * k);
+                        const float4 x1 = *cell(row + q * (TILE >> copies), 2 * k + 1);
+                        o[0] += x0.x, o[1] += x0.y, o[2] += x0.z, o[3] += x0.w;
+                        o[4] += x1.x, o[5] += x1.y, o[6] += x1.z, o[7] += x1.w;
+                    }
+                    if (whole) {
+                        store8_bf16(out_row<HD>(p, d, lead + row) + c + 8 * k, o, p.a.out_pair_order);
+                    } else {
+                        float4 *dst = reinterpret_cast<float4 *>(rec + (lead + row) * HD + c + 8 * k);
+                        dst[0] = make_float4(o[0], o[1], o[2], o[3]);
+                        dst[1] = make_float4(o[4], o[5], o[6], o[7]);
+                    }
+                }
+                named_bar_sync(2 + st, 128);
+            }
+            if (__any_sync(0xffffffffu, odd[lane & 7] != 0u) && mine && copy == 0)
+                add_odd_values(p, d, mask, odd, dim0, dim1, whole ? nullptr : rec + rr * HD, out_row<HD>(p, d, rr));
+            if (!whole && mine && copy == 0 && dim0 == 0) {
+                rec[ROWS * HD + rr] = top;
+                rec[ROWS * HD + ROWS + rr] = lsum;
             }
             tc_fence_before();
             __syncwarp();
@@ -734,127 +859,121 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                 if (both) mbar_arrive(&q_empty[1]);
             }
             if (!whole) {
-                if (mine && copy == 0 && dim0 == 0) {
-                    float *ml = rec - rr * HD + ROWS * HD + rr;
-                    ml[0] = top;
-                    ml[ROWS] = lsum;
-                }
                 shares[d.t0 == 0] = true;
                 if (tid == 0) shared_units[d.t0 == 0] = d;
-                asm volatile("fence.acq_rel.gpu;" ::: "memory");
                 named_bar_sync(1, SOFTMAX_THREADS);
-                if (tid == 0) atomicAdd(&p.arrived[d.owner0], 1u);
+                if (tid == 0) {  // the barrier's order and this fence publish all threads' stores
+                    asm volatile("fence.acq_rel.gpu;" ::: "memory");
+                    atomicAdd(&p.arrived[division->owner(d.start)], 1u);
+                }
             }
         }
-        // Merge the shared units: this CTA's share of their rows.  A warp
-        // takes a row and a part of the unit's pieces.
+        // Merge the shared units: this CTA's share of their rows.  A thread
+        // takes 8 dims of a row and a part of the unit's pieces.
 #pragma unroll 1
         for (int which = 0; which < 2; ++which) {
             if (!shares[which]) continue;
             const Piece u = shared_units[which];
-            const int k = u.ctas, me = blockIdx.x - u.owner0;
-            const int r0 = u.rows * me / k, r1 = u.rows * (me + 1) / k;
-            if (r1 > r0) {
-                bool ok = true;
+            const int owner0 = division->owner(u.start), k = division->owner(u.start + u.nt - 1) - owner0 + 1;
+            const int me = blockIdx.x - owner0;
+            const int r0 = u.rows * me / k, rows = u.rows * (me + 1) / k - r0;
+            bool ok = true;
+            if (rows > 0) {
                 if (lane == 0) {
                     const uint64_t since = globaltimer();
-                    while (ok && *reinterpret_cast<volatile unsigned *>(&p.arrived[u.owner0]) != static_cast<unsigned>(k))
+                    while (ok && *reinterpret_cast<volatile unsigned *>(&p.arrived[owner0]) != static_cast<unsigned>(k))
                         if (*abort || globaltimer() - since > kArrivalWaitNs) {
                             atomicExch(p.status, static_cast<unsigned>(DEV_TIMEOUT));
                             ok = false;
                         }
+                    asm volatile("fence.acq_rel.gpu;" ::: "memory");
                 }
                 ok = __all_sync(0xffffffffu, ok);
-                asm volatile("fence.acq_rel.gpu;" ::: "memory");
-                constexpr int W = HD / 32;
-                // Warps of a row: as many as there are for the share's rows, each with at least two pieces.
-                int parts = 1;
-                while (2 * parts * (r1 - r0) <= SOFTMAX_WARPS && 4 * parts <= k) parts *= 2;
-                const int part = warp % parts;
-                float *ex = reinterpret_cast<float *>(ring);  // no copies are in flight any more
+            }
+            // Every warp of the unit's CTAs counts itself once it has seen all
+            // arrivals; the last clears the counters for the next launch.
+            unsigned seen = 0;
+            if (lane == 0) seen = atomicAdd(&p.done[owner0], 1u);
+            constexpr int CHUNKS = HD / 8;
+            int parts = 1;  // as many threads for a row's 8 dims as there are, each with at least two pieces
+            while (2 * parts * rows * CHUNKS <= SOFTMAX_THREADS && 4 * parts <= k) parts *= 2;
+            const int c = tid % CHUNKS, part = tid / CHUNKS % parts, step = SOFTMAX_THREADS / CHUNKS / parts;
+            float *ex = reinterpret_cast<float *>(ring);  // no copies are in flight any more
 #pragma unroll 1
-                for (int base = r0; base < r1; base += SOFTMAX_WARPS / parts) {
-                    const int rr = base + warp / parts;
-                    const bool on = ok && rr < r1;
-                    float top = -INFINITY, lsum = 0.0f, o[W];
-#pragma unroll
-                    for (int e = 0; e < W; ++e) o[e] = 0.0f;
-                    if (on) {
-                        const int j1 = k * (part + 1) / parts;
+            for (int base = 0; base < rows; base += step) {
+                const int row = base + tid / CHUNKS / parts, rr = r0 + row;
+                const bool on = ok && row < rows;
+                float top = -INFINITY, lsum = 0.0f, o[8] = {};
+                if (on) {
+                    const int j1 = k * (part + 1) / parts;
 #pragma unroll 1
-                        for (int j0 = k * part / parts; j0 < j1; j0 += 4) {
-                            float mj[4], lj[4], q[4][W];
+                    for (int j0 = k * part / parts; j0 < j1; j0 += 4) {
+                        float mj[4], lj[4];
+                        float4 q[4][2];
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {  // every load of four pieces first
-                                const int j = min(j0 + i, j1 - 1);
-                                const float *rec = p.partial + (2 * static_cast<int64_t>(u.owner0 + j) + (j == 0)) * C::RECORD;
-                                mj[i] = j0 + i < j1 ? __ldcg(rec + ROWS * HD + rr) : -INFINITY;
-                                lj[i] = __ldcg(rec + ROWS * HD + ROWS + rr);
-                                if (W == 4) *reinterpret_cast<float4 *>(q[i]) = __ldcg(reinterpret_cast<const float4 *>(rec + rr * HD) + lane);
-                                else *reinterpret_cast<float2 *>(q[i]) = __ldcg(reinterpret_cast<const float2 *>(rec + rr * HD) + lane);
-                            }
-                            const float t = fmaxf(fmaxf(fmaxf(mj[0], mj[1]), fmaxf(mj[2], mj[3])), top);
-                            const float keep = top == -INFINITY ? 0.0f : exp2_approx(top - t);
-                            top = t;
-                            lsum *= keep;
-#pragma unroll
-                            for (int e = 0; e < W; ++e) o[e] *= keep;
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const float wt = mj[i] == -INFINITY ? 0.0f : exp2_approx(mj[i] - t);
-                                if (wt != 0.0f) {
-                                    lsum = fmaf(lj[i], wt, lsum);
-#pragma unroll
-                                    for (int e = 0; e < W; ++e) o[e] = fmaf(q[i][e], wt, o[e]);
-                                }
-                            }
+                        for (int i = 0; i < 4; ++i) {  // every load of four pieces first
+                            const int j = min(j0 + i, j1 - 1);
+                            const float *rec = p.partial + (2 * static_cast<int64_t>(owner0 + j) + (j == 0)) * C::RECORD;
+                            mj[i] = j0 + i < j1 ? __ldcg(rec + ROWS * HD + rr) : -INFINITY;
+                            lj[i] = __ldcg(rec + ROWS * HD + ROWS + rr);
+                            const float4 *src = reinterpret_cast<const float4 *>(rec + rr * HD) + 2 * c;
+                            q[i][0] = __ldcg(src);
+                            q[i][1] = __ldcg(src + 1);
                         }
-                    }
-                    if (parts > 1) {  // join the parts, in order, in the row's first warp
-                        float *my = ex + warp * (HD + 2);
-                        named_bar_sync(1, SOFTMAX_THREADS);
+                        const float t = fmaxf(fmaxf(fmaxf(mj[0], mj[1]), fmaxf(mj[2], mj[3])), top);
+                        const float keep = top == -INFINITY ? 0.0f : exp2_approx(top - t);
+                        top = t;
+                        lsum *= keep;
 #pragma unroll
-                        for (int e = 0; e < W; ++e) my[lane * W + e] = o[e];
-                        if (lane == 0) my[HD] = top, my[HD + 1] = lsum;
-                        named_bar_sync(1, SOFTMAX_THREADS);
-                        if (part == 0) {
-#pragma unroll 1
-                            for (int i = 1; i < parts; ++i) top = fmaxf(top, my[i * (HD + 2) + HD]);
-                            lsum = 0.0f;
+                        for (int e = 0; e < 8; ++e) o[e] *= keep;
 #pragma unroll
-                            for (int e = 0; e < W; ++e) o[e] = 0.0f;
-#pragma unroll 1
-                            for (int i = 0; i < parts; ++i) {
-                                const float *q = my + i * (HD + 2);
-                                const float wt = q[HD] == -INFINITY ? 0.0f : exp2_approx(q[HD] - top);
-                                if (wt != 0.0f) {
-                                    lsum = fmaf(q[HD + 1], wt, lsum);
-#pragma unroll
-                                    for (int e = 0; e < W; ++e) o[e] = fmaf(q[lane * W + e], wt, o[e]);
-                                }
+                        for (int i = 0; i < 4; ++i)
+                            if (mj[i] != -INFINITY) {
+                                const float wt = exp2_approx(mj[i] - t);
+                                lsum = fmaf(lj[i], wt, lsum);
+                                o[0] = fmaf(q[i][0].x, wt, o[0]), o[1] = fmaf(q[i][0].y, wt, o[1]);
+                                o[2] = fmaf(q[i][0].z, wt, o[2]), o[3] = fmaf(q[i][0].w, wt, o[3]);
+                                o[4] = fmaf(q[i][1].x, wt, o[4]), o[5] = fmaf(q[i][1].y, wt, o[5]);
+                                o[6] = fmaf(q[i][1].z, wt, o[6]), o[7] = fmaf(q[i][1].w, wt, o[7]);
                             }
-                        }
                     }
-                    if (on && part == 0) {
-                        const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
-                        const int x = u.row0 + rr, node = x / p.group, g = x - node * p.group;
-                        uint16_t *dst = p.a.out + (static_cast<int64_t>(u.first) + node) * p.a.ld_out +
-                                        (static_cast<int64_t>(u.kv) * p.group + g) * HD;
+                }
+                if (parts > 1) {  // join the parts, in order, in the row's first
+                    float *my = ex + tid;  // value e of a thread at ex[e * threads + thread]
+                    named_bar_sync(1, SOFTMAX_THREADS);
 #pragma unroll
-                        for (int e = 0; e < W; ++e) {
-                            const int dim = lane * W + e, in8 = dim & 7;
-                            const int col = p.a.out_pair_order ? (dim & ~7) + (in8 < 4 ? 2 * in8 : 2 * (in8 - 4) + 1) : dim;
-                            dst[col] = f32_to_bf16_bits(o[e] * inv);
+                    for (int e = 0; e < 8; ++e) my[e * SOFTMAX_THREADS] = o[e];
+                    my[8 * SOFTMAX_THREADS] = top, my[9 * SOFTMAX_THREADS] = lsum;
+                    named_bar_sync(1, SOFTMAX_THREADS);
+                    if (part == 0) {
+#pragma unroll 1
+                        for (int i = 1; i < parts; ++i) top = fmaxf(top, my[8 * SOFTMAX_THREADS + i * CHUNKS]);
+                        lsum = 0.0f;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) o[e] = 0.0f;
+#pragma unroll 1
+                        for (int i = 0; i < parts; ++i) {
+                            const float mi = my[8 * SOFTMAX_THREADS + i * CHUNKS];
+                            if (mi == -INFINITY) continue;
+                            const float wt = exp2_approx(mi - top);
+                            lsum = fmaf(my[9 * SOFTMAX_THREADS + i * CHUNKS], wt, lsum);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) o[e] = fmaf(my[e * SOFTMAX_THREADS + i * CHUNKS], wt, o[e]);
                         }
                     }
                 }
+                if (on && part == 0) {
+                    const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) o[e] *= inv;
+                    store8_bf16(out_row<HD>(p, u, rr) + 8 * c, o, p.a.out_pair_order);
+                }
             }
-            // The last of the unit's CTAs clears its counters for the next launch.
-            named_bar_sync(1, SOFTMAX_THREADS);
-            if (tid == 0 && atomicAdd(&p.done[u.owner0], 1u) == static_cast<unsigned>(k - 1)) {
-                atomicExch(&p.arrived[u.owner0], 0u);
-                atomicExch(&p.done[u.owner0], 0u);
+            if (lane == 0 && seen == static_cast<unsigned>(k * SOFTMAX_WARPS - 1)) {
+                atomicExch(&p.arrived[owner0], 0u);
+                atomicExch(&p.done[owner0], 0u);
             }
+            named_bar_sync(1, SOFTMAX_THREADS);  // the next unit uses `ex` again
         }
     }
     tc_fence_before();
