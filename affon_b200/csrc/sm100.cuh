@@ -111,18 +111,33 @@ AFB_DEVICE void tma_load_2d_hint(void *smem_dst, const CUtensorMap *map, uint64_
         "l"(policy)
         : "memory");
 }
-// 4D tiled TMA load with an L2 cache policy, issued by a whole converged warp
-// (its leader's counts).
-AFB_DEVICE void tma_load_4d_elect(void *smem_dst, const CUtensorMap *map, uint64_t *bar, int c0, int c1, int c2, int c3,
-                                 uint64_t policy) {
-    asm volatile(
-        "{\n\t.reg .pred e;\n\t"
-        "elect.sync _|e, 0xffffffff;\n\t"
-        "@e cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
-        " [%0], [%1, {%3, %4, %5, %6}], [%2], %7;\n\t}"
-        ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2),
-        "r"(c3), "l"(policy)
-        : "memory");
+// 4D tiled TMA loads with an L2 cache policy, issued by a whole converged warp
+// (its leader's count): RUNS boxes side by side along the innermost axis, 64
+// 16-bit elements and `step` bytes of shared memory apart.
+template <int RUNS>
+AFB_DEVICE void tma_load_4d_elect(uint32_t smem_dst, uint32_t step, const CUtensorMap *map, uint64_t *bar, int c1, int c2,
+                                  int c3, uint64_t policy) {
+    if constexpr (RUNS == 2)
+        asm volatile(
+            "{\n\t.reg .pred e;\n\t.reg .b32 d;\n\t"
+            "elect.sync _|e, 0xffffffff;\n\t"
+            "@e cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+            " [%0], [%1, {0, %3, %4, %5}], [%2], %6;\n\t"
+            "add.u32 d, %0, %7;\n\t"
+            "@e cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+            " [d], [%1, {64, %3, %4, %5}], [%2], %6;\n\t}"
+            ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c1), "r"(c2), "r"(c3),
+            "l"(policy), "r"(step)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred e;\n\t"
+            "elect.sync _|e, 0xffffffff;\n\t"
+            "@e cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+            " [%0], [%1, {0, %3, %4, %5}], [%2], %6;\n\t}"
+            ::"r"(smem_dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c1), "r"(c2), "r"(c3),
+            "l"(policy)
+            : "memory");
 }
 AFB_DEVICE uint64_t l2_evict_normal() {
     uint64_t policy;
@@ -196,19 +211,6 @@ AFB_DEVICE uint64_t umma_desc_sw128(uint32_t smem_addr) {
     return d;
 }
 
-// The same for an operand whose M or N axis is contiguous (MN-major): 64
-// elements (128 B) per row of the K axis, 8-row atoms of 1024 B along K
-// (stride byte offset), `mn_bytes` between runs of 64 M or N elements (leading
-// byte offset).  A 16-element K step is 2048 B.
-AFB_DEVICE uint64_t umma_desc_mn_sw128(uint32_t smem_addr, uint32_t mn_bytes) {
-    uint64_t d = 0;
-    d |= static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu);
-    d |= static_cast<uint64_t>(mn_bytes >> 4) << 16;
-    d |= static_cast<uint64_t>(1024u >> 4) << 32;
-    d |= static_cast<uint64_t>(1u) << 46;
-    d |= static_cast<uint64_t>(2u) << 61;
-    return d;
-}
 // Instruction descriptor bits: B is MN-major; A enters negated.
 constexpr uint32_t kUmmaTransposeB = 1u << 16, kUmmaNegateA = 1u << 13;
 
@@ -231,29 +233,64 @@ AFB_DEVICE void umma_bf16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, 
         : "memory");
 }
 
-// The same issued by a whole converged warp, whose leader's instruction counts
-// (elect.sync names the same lane every time, so its commit covers them):
-// with the operands warp-uniform the compiler keeps them in uniform registers,
-// where a branch on the lane costs a move per operand.
-AFB_DEVICE void umma_bf16_ss_elect(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                   uint32_t accumulate) {
+// Runs of MMAs and their commit, issued by a whole converged warp whose
+// leader's instructions count (elect.sync names the same lane every time, so
+// its commits cover them).  One election and few instructions per run matter:
+// the issuing warp has only its own instruction latency to work with.
+//
+// D (128 x N) = A (128 x 16 STEPS) B, both K-major with the 128-byte swizzle
+// (64 K elements per 16 KB): descriptors as lo words (umma_lo) and kUmmaHi.
+constexpr uint32_t kUmmaHi = (1024u >> 4) | (1u << 14) | (2u << 29);  // stride 1024 B, version 1, SWIZZLE_128B
+AFB_DEVICE uint32_t umma_lo(uint32_t smem_addr, uint32_t leading_bytes) {
+    return ((smem_addr >> 4) & 0x3FFFu) | ((leading_bytes >> 4) << 16);
+}
+#define AFB_MMA_SS(off, acc) \
+    "add.u32 al, %1, " off "; add.u32 bl, %2, " off "; mov.b64 ad, {al, %3}; mov.b64 bd, {bl, %3};\n\t" \
+    "@e tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %4, " acc ";\n\t"
+template <int STEPS>
+AFB_DEVICE void umma_run_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint64_t *bar) {
+    if constexpr (STEPS == 8)
+        asm volatile(
+            "{\n\t.reg .pred e, t, f;\n\t.reg .b32 al, bl;\n\t.reg .b64 ad, bd;\n\t"
+            "elect.sync _|e, 0xffffffff;\n\tsetp.eq.u32 t, 0, 0;\n\tsetp.ne.u32 f, 0, 0;\n\t"
+            AFB_MMA_SS("0", "f") AFB_MMA_SS("2", "t") AFB_MMA_SS("4", "t") AFB_MMA_SS("6", "t")
+            AFB_MMA_SS("1024", "t") AFB_MMA_SS("1026", "t") AFB_MMA_SS("1028", "t") AFB_MMA_SS("1030", "t")
+            "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%5];\n\t}"
+            ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(kUmmaHi), "r"(idesc), "r"(smem_u32(bar))
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred e, t, f;\n\t.reg .b32 al, bl;\n\t.reg .b64 ad, bd;\n\t"
+            "elect.sync _|e, 0xffffffff;\n\tsetp.eq.u32 t, 0, 0;\n\tsetp.ne.u32 f, 0, 0;\n\t"
+            AFB_MMA_SS("0", "f") AFB_MMA_SS("2", "t") AFB_MMA_SS("4", "t") AFB_MMA_SS("6", "t")
+            "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%5];\n\t}"
+            ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(kUmmaHi), "r"(idesc), "r"(smem_u32(bar))
+            : "memory");
+}
+#undef AFB_MMA_SS
+// D += A B for 64 K elements (D = A B when !accumulate): A from tensor memory
+// (lane = row, a 32-bit column = two consecutive K elements), B MN-major (its
+// N axis contiguous, 128-byte swizzle, 16 K rows per 2048 B).
+#define AFB_MMA_TS(col, off, acc) \
+    "add.u32 al, %1, " col "; add.u32 bl, %2, " off "; mov.b64 bd, {bl, %3};\n\t" \
+    "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [al], bd, %4, " acc ";\n\t"
+AFB_DEVICE void umma_run_ts4(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p, e;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "elect.sync _|e, 0xffffffff;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred e, t, f;\n\t.reg .b32 al, bl;\n\t.reg .b64 bd;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\tsetp.eq.u32 t, 0, 0;\n\tsetp.ne.u32 f, %5, 0;\n\t"
+        AFB_MMA_TS("0", "0", "f") AFB_MMA_TS("8", "128", "t") AFB_MMA_TS("16", "256", "t") AFB_MMA_TS("24", "384", "t")
+        "}"
+        ::"r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(kUmmaHi), "r"(idesc), "r"(accumulate)
         : "memory");
 }
-// A from tensor memory: lane = row, a 32-bit column = two consecutive K elements.
-AFB_DEVICE void umma_bf16_ts_elect(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                   uint32_t accumulate) {
+#undef AFB_MMA_TS
+// One 16-element step of it.
+AFB_DEVICE void umma_step_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p, e;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "elect.sync _|e, 0xffffffff;\n\t"
-        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred e, f;\n\t.reg .b64 bd;\n\t"
+        "elect.sync _|e, 0xffffffff;\n\tsetp.ne.u32 f, %5, 0;\n\tmov.b64 bd, {%2, %3};\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], bd, %4, f;\n\t}"
+        ::"r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(kUmmaHi), "r"(idesc), "r"(accumulate)
         : "memory");
 }
 AFB_DEVICE void umma_commit_elect(uint64_t *bar) {

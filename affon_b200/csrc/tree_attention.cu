@@ -108,7 +108,6 @@ struct Piece {
     int seq, first, n, ctx, kv, row0, rows, t0, t1, nt;
     int start;  // the unit's first tile in the order of all tiles
     __device__ __forceinline__ bool both() const { return rows > TILE; }  // two row tiles, every position tile for both
-    __device__ __forceinline__ int items() const { return both() ? 2 * (t1 - t0) : t1 - t0; }
     // log2 of the copies of the rows in the 128 rows of the MMA.
     __device__ __forceinline__ int copies() const { return rows <= 32 ? 2 : rows <= 64 ? 1 : 0; }
 };
@@ -294,10 +293,10 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
     char *ring = qbuf + 2 * C::TILE_BYTES;
     uint64_t *full = reinterpret_cast<uint64_t *>(ring + C::STAGES * C::TILE_BYTES);
     uint64_t *empty = full + C::STAGES;
-    uint64_t *s_full = empty + C::STAGES;  // [2] scores of a stream are in tensor memory
-    uint64_t *p_half = s_full + 2;         // [2] probabilities of a tile's first 64 positions are
-    uint64_t *p_full = p_half + 2;         // [2] the rest
-    uint64_t *q_full = p_full + 2;         // [2] query buffers
+    uint64_t *s_full = empty + C::STAGES;  // [2 streams][2 halves] scores are in tensor memory
+    uint64_t *p_full = s_full + 4;         // [2][2] probabilities are
+    uint64_t *pv_done = p_full + 4;        // [2] a half's product is in O
+    uint64_t *q_full = pv_done + 2;        // [2] query buffers
     uint64_t *q_empty = q_full + 2;
     uint64_t *d_full = q_empty + 2;        // [PIECES] the queue
     uint64_t *d_empty = d_full + PIECES;
@@ -318,9 +317,11 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
             mbar_init(&empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&s_full[i], 1);
-            mbar_init(&p_half[i], 128);
-            mbar_init(&p_full[i], 128);
+            mbar_init(&s_full[2 * i], 1);
+            mbar_init(&s_full[2 * i + 1], 1);
+            mbar_init(&p_full[2 * i], SOFTMAX_WARPS / 2);
+            mbar_init(&p_full[2 * i + 1], SOFTMAX_WARPS / 2);
+            mbar_init(&pv_done[i], 1);
             mbar_init(&q_full[i], 1);
             mbar_init(&q_empty[i], SOFTMAX_WARPS);
         }
@@ -461,9 +462,11 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
             }
         }
     } else if (warp == PRODUCER) {  // --------------------------------------------- K and V tiles
-        const int shift = p.s.page_shift, rows_per_box = min(1 << shift, TILE);
+        const int shift = p.s.page_shift, box_shift = min(shift, 7), rows_per_box = 1 << box_shift;
         const uint64_t once = l2_evict_first(), again = l2_evict_normal();
-        uint32_t seq_no = 0;  // ring position, over all pieces
+        const uint32_t ring_addr = smem_u32(ring);
+        int next = 0;  // the ring's next stage, over all pieces
+        uint32_t next_phase = 0, sent = 0, phases = 0;
         Piece d;
         while (next_piece(d)) {
             const int *table = p.t.page_table + d.seq * p.s.ld_table;
@@ -474,31 +477,34 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
             // them; the second half is fetched while the first is used.
             const int last_page = (len - 1) >> shift;
             int page0 = (t0 * TILE) >> shift;
-            auto fetch = [&](int i) { return table[min(i + lane, last_page)]; };
+            auto fetch = [&](int i) {
+                int page = table[min(i + lane, last_page)];
+                if (page < 0 || page >= p.s.pages) {  // a coordinate outside the map reads zeros
+                    if (i + lane <= last_page) atomicExch(p.status, static_cast<unsigned>(DEV_BOUNDS));
+                    page = static_cast<int>(p.s.pages);
+                }
+                return page;
+            };
             int ids = fetch(page0), more = fetch(page0 + 32);
             auto load = [&](const CUtensorMap *map, int t) {
-                const int pos = t * TILE, boxes = (min(TILE, len - pos) + rows_per_box - 1) / rows_per_box;
-                const int stage = seq_no % C::STAGES;
-                if (!warp_wait(&empty[stage], ((seq_no / C::STAGES) & 1) ^ 1, abort, p.status) ||
-                    __any_sync(0xffffffffu, *abort))
+                const int pos = t * TILE, boxes = (min(TILE, len - pos) + rows_per_box - 1) >> box_shift;
+                const int stage = next;
+                if (!warp_wait(&empty[stage], next_phase ^ 1, abort, p.status) || __any_sync(0xffffffffu, *abort))
                     return;  // never re-arm a stage after an abort
                 if (lane == 0) mbar_arrive_expect_tx(&full[stage], boxes * C::HALVES * rows_per_box * 128);
                 __syncwarp();
-                char *dst = ring + stage * C::TILE_BYTES;
-#pragma unroll 1
+                const uint32_t dst = ring_addr + stage * C::TILE_BYTES;
+                const int first = (pos >> shift) - page0, row = pos & ((1 << shift) - 1);
+#pragma unroll 4
                 for (int b = 0; b < boxes; ++b) {
-                    const int i = ((pos + b * rows_per_box) >> shift) - page0;
-                    int page = uniform(__shfl_sync(0xffffffffu, i < 32 ? ids : more, i & 31));
-                    if (page < 0 || page >= p.s.pages) {  // a coordinate outside the map reads zeros
-                        if (lane == 0) atomicExch(p.status, static_cast<unsigned>(DEV_BOUNDS));
-                        page = static_cast<int>(p.s.pages);
-                    }
-#pragma unroll
-                    for (int h = 0; h < C::HALVES; ++h)
-                        tma_load_4d_elect(dst + h * HALF_BYTES + b * rows_per_box * 128, map, &full[stage], h * 64,
-                                          pos & ((1 << shift) - 1), kv, page, policy);
+                    const int i = first + b;
+                    const int page = __shfl_sync(0xffffffffu, i < 32 ? ids : more, i & 31);
+                    tma_load_4d_elect<C::HALVES>(dst + b * rows_per_box * 128, HALF_BYTES, map, &full[stage], row, kv, page,
+                                                 policy);
                 }
-                ++seq_no;
+                sent |= 1u << stage;
+                phases = (phases & ~(1u << stage)) | next_phase << stage;
+                if (++next == C::STAGES) next = 0, next_phase ^= 1;
             };
             // The order in which the MMA warp consumes them: with two row
             // tiles K0 V0 K1 V1 .., else K0 K1 V0 K2 V1 .. (a tile's values
@@ -516,98 +522,122 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
             }
         }
         // Copies in flight land before the CTA leaves.
-        for (uint32_t back = 1; back <= C::STAGES && back <= seq_no; ++back) {
-            const uint32_t i = seq_no - back;
-            mbar_wait_drain(&full[i % C::STAGES], (i / C::STAGES) & 1);
-        }
+        for (int i = 0; i < C::STAGES; ++i)
+            if (sent >> i & 1) mbar_wait_drain(&full[i], phases >> i & 1);
     } else if (warp == MMA) {  // ---------------------------------------------------- tensor cores
         // A negative scale negates the queries, so the running maximum can
         // work on the scores as they come.
-        const uint32_t idesc_s = umma_idesc_bf16(128, TILE) | (p.a.scale < 0.0f ? kUmmaNegateA : 0u);
+        const uint32_t negate = p.a.scale < 0.0f ? kUmmaNegateA : 0u;
+        const uint32_t idesc_s = umma_idesc_bf16(128, TILE) | negate, idesc_h = umma_idesc_bf16(128, TILE / 2) | negate;
         const uint32_t idesc_o = umma_idesc_bf16(128, HD) | kUmmaTransposeB;
-        const uint32_t q_addr = smem_u32(qbuf), ring_addr = smem_u32(ring);
-        uint32_t base = 0, p_phase = 0, pieces = 0;
+        const uint32_t q_lo = umma_lo(smem_u32(qbuf), 16), k_lo = umma_lo(smem_u32(ring), 16);
+        const uint32_t v_lo = umma_lo(smem_u32(ring), HALF_BYTES);
+        constexpr uint32_t TILE_LO = C::TILE_BYTES >> 4, SUB_LO = 64 * 128 >> 4;  // a tile, 64 positions of it
+        int next = 0;  // the ring's next stage: tiles are used in the order in which they are loaded
+        uint32_t next_phase = 0, p_phase = 0, pieces = 0;
         bool live = true;
         QuerySlots slots;
         Piece d;
         while (live && next_piece(d)) {
-            const int nt = uniform(d.t1 - d.t0), both = uniform(d.both()), items = both ? 2 * nt : nt;
-            const bool halves = uniform(d.copies() == 0);  // P comes in two halves
+            const int nt = uniform(d.t1 - d.t0), both = uniform(d.both());
             const int tile0 = uniform(d.t0), ctx = uniform(d.ctx), len = uniform(d.ctx + d.n);
             const int slot = uniform(slots.take(both));
             live = warp_wait(&q_full[slot], slots.parity(slot), abort, p.status);
             if (live && both) live = warp_wait(&q_full[1], slots.parity(1), abort, p.status);
             if (!live) break;
-            auto scores = [&](int w) {
-                const int t = both ? w >> 1 : w, st = w & 1;
-                const uint32_t no = base + (both ? 2 * t : t == 0 ? 0 : 2 * t - 1);
-                const int stage = no % C::STAGES;
-                if (!both || st == 0) live = warp_wait(&full[stage], (no / C::STAGES) & 1, abort, p.status);
-                if (!live) return;
-                const uint64_t a = umma_desc_sw128(q_addr + (both ? st : slot) * C::TILE_BYTES);
-                const uint64_t b = umma_desc_sw128(ring_addr + stage * C::TILE_BYTES);
-#pragma unroll
-                for (int ks = 0; ks < HD / 16; ++ks) {  // the descriptors' addresses count 16 bytes
-                    const uint32_t off = ((ks >> 2) * HALF_BYTES + (ks & 3) * 32) >> 4;
-                    umma_bf16_ss_elect(tmem + st * TILE, a + off, b + off, idesc_s, ks > 0);
-                }
-                umma_commit_elect(&s_full[st]);
-                if (!both || st == 1) umma_commit_elect(&empty[stage]);
+            auto take = [&]() {  // waits for the next stage to land
+                const int stage = next;
+                live = live && warp_wait(&full[stage], next_phase, abort, p.status);
+                if (++next == C::STAGES) next = 0, next_phase ^= 1;
+                return stage;
             };
-            auto values = [&](int w) {
-                const int t = both ? w >> 1 : w, st = w & 1;
-                const uint32_t no = base + (both ? 2 * t + 1 : t == nt - 1 ? 2 * nt - 1 : 2 * t + 2);
-                const int stage = no % C::STAGES;
-                if (w == 0) {  // the last piece's O and `odd` have been read
-                    if (pieces) live = warp_wait(o_free, (pieces - 1) & 1, abort, p.status);
-                    if (!live) return;
-                    if (lane < kMaxTreeNodes / 32) odd[lane] = 0u;
-                    __syncwarp();
-                }
-                const int pos = (tile0 + t) * TILE, valid = min(TILE, len - pos);
-                if (!both || st == 0) {
-                    live = warp_wait(&full[stage], (no / C::STAGES) & 1, abort, p.status);
-                    if (!live) return;
-                    if (pos + TILE > ctx)
-                        clean_values<HD>(ring + stage * C::TILE_BYTES, max(0, ctx - pos), valid, pos - ctx, odd);
-                }
-                // 16 positions a step; steps behind the last position are left out.
-                const int steps = (valid + 15) >> 4;
-                const uint64_t b = umma_desc_mn_sw128(ring_addr + stage * C::TILE_BYTES, HALF_BYTES);
-                auto product = [&](int ks) {
-                    if (ks < steps)
-                        umma_bf16_ts_elect(tmem + 2 * TILE + st * HD, tmem + st * TILE + ks * 8, b + ks * (2048 >> 4),
-                                           idesc_o, w >= 2 || ks > 0);
-                };
-                if (halves) {
-                    live = warp_wait(&p_half[st], (p_phase >> (2 + st)) & 1, abort, p.status);
-                    p_phase ^= 4u << st;
-                    if (!live) return;
-                    tc_fence_after();
-#pragma unroll
-                    for (int ks = 0; ks < 4; ++ks) product(ks);
-                }
-                live = warp_wait(&p_full[st], (p_phase >> st) & 1, abort, p.status);
-                p_phase ^= 1u << st;
-                if (!live) return;
+            auto p_ready = [&](int i) {
+                live = live && warp_wait(&p_full[i], (p_phase >> i) & 1, abort, p.status);
+                p_phase ^= 1u << i;
                 tc_fence_after();
-                if (!halves) {
-#pragma unroll
-                    for (int ks = 0; ks < 4; ++ks) product(ks);
+            };
+            // A tile's values have landed; returns the 16-position steps that hold any of its positions.
+            auto enter = [&](int t, int stage) {
+                const int pos = (tile0 + t) * TILE, valid = min(TILE, len - pos);
+                if (live && pos + TILE > ctx)
+                    clean_values<HD>(ring + stage * C::TILE_BYTES, max(0, ctx - pos), valid, pos - ctx, odd);
+                return (valid + 15) >> 4;
+            };
+            // O += P V of 64 positions, `steps` of their 4 steps.
+            auto values = [&](int st, uint32_t p_tmem, uint32_t lo, int steps, bool accumulate) {
+                const uint32_t o = tmem + 2 * TILE + st * HD;
+                if (steps >= 4) {
+                    umma_run_ts4(o, p_tmem, lo, idesc_o, accumulate);
+                } else {
+#pragma unroll 1
+                    for (int ks = 0; ks < steps; ++ks)
+                        umma_step_ts(o, p_tmem + 8 * ks, lo + 128 * ks, idesc_o, accumulate || ks > 0);
                 }
-#pragma unroll
-                for (int ks = 4; ks < TILE / 16; ++ks) product(ks);
-                if (!both || st == 1) umma_commit_elect(&empty[stage]);
             };
 #pragma unroll 1
-            for (int w = -2; w < items && live; ++w) {
-                if (w >= 0) values(w);
-                if (live && w + 2 < items) scores(w + 2);
+            for (int t = 0; t < (both ? 1 : 2) && t < nt; ++t) {
+                const int k = take();
+                if (!live) break;
+                const uint32_t lo = k_lo + k * TILE_LO;
+                if (both) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        umma_run_ss<HD / 16>(tmem + (i & 1) * TILE + (i >> 1) * 64, q_lo + (i & 1) * TILE_LO,
+                                             lo + (i >> 1) * SUB_LO, idesc_h, &s_full[2 * (i & 1) + (i >> 1)]);
+                } else {
+                    umma_run_ss<HD / 16>(tmem + t * TILE, q_lo + slot * TILE_LO, lo, idesc_s, &s_full[2 * t]);
+                }
+                umma_commit_elect(&empty[k]);
             }
+            if (pieces && live) live = warp_wait(o_free, (pieces - 1) & 1, abort, p.status);
+            if (!live) break;
+            if (lane < kMaxTreeNodes / 32) odd[lane] = 0u;  // the last piece's have been read
+            __syncwarp();
+#pragma unroll 1
+            for (int t = 0; t < nt && live; ++t) {
+                const int v = take();
+                const int steps = enter(t, v);
+                const uint32_t lo = v_lo + v * TILE_LO;
+                if (both) {
+                    const bool more = t + 1 < nt;
+                    int k = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int st = i & 1, h = i >> 1;
+                        p_ready(2 * st + h);
+                        if (!live) break;
+                        values(st, tmem + st * TILE + h * 64, lo + h * SUB_LO, steps - 4 * h, t > 0 || h > 0);
+                        umma_commit_elect(&pv_done[st]);
+                        if (more) {
+                            if (i == 0) k = take();
+                            if (!live) break;
+                            umma_run_ss<HD / 16>(tmem + st * TILE + h * 64, q_lo + st * TILE_LO,
+                                                 k_lo + k * TILE_LO + h * SUB_LO, idesc_h, &s_full[2 * st + h]);
+                        }
+                    }
+                    if (!live) break;
+                    umma_commit_elect(&empty[v]);
+                    if (more) umma_commit_elect(&empty[k]);
+                } else {
+                    const int st = t & 1;
+                    p_ready(2 * st);
+                    if (!live) break;
+                    values(st, tmem + st * TILE, lo, steps, t >= 2);
+                    values(st, tmem + st * TILE + 32, lo + SUB_LO, steps - 4, true);
+                    umma_commit_elect(&empty[v]);
+                    if (t + 2 < nt) {
+                        const int k = take();
+                        if (!live) break;
+                        umma_run_ss<HD / 16>(tmem + st * TILE, q_lo + slot * TILE_LO, k_lo + k * TILE_LO, idesc_s,
+                                             &s_full[2 * st]);
+                        umma_commit_elect(&empty[k]);
+                    }
+                }
+            }
+            if (!live) break;
             __syncwarp();
             if (lane == 0) mbar_arrive(unit_done);  // `odd` is written
             umma_commit_elect(unit_done);
-            base += 2 * nt;
             ++pieces;
         }
         // On the way out of an abort, MMAs in flight end before tensor memory is freed.
@@ -618,9 +648,9 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
     } else {  // ------------------------------------------------------------------------ softmax
         const int st = warp >> 2, r = tid & 127;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t ts = tmem + lanes + st * TILE, to = tmem + lanes + 2 * TILE;
+        const uint32_t to = tmem + lanes + 2 * TILE;
         const float sc = fabsf(p.a.scale) * LOG2E;
-        uint32_t s_phase = 0, u_phase = 0;
+        uint32_t s_phase = 0, u_phase = 0, products = 0;
         bool shares[2] = {false, false};
         QuerySlots slots;
         Piece d;
@@ -640,17 +670,23 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                 named_bar_sync(2 + st, 128);
                 if (r == 0) mbar_arrive(&q_full[st]);
             }
-            const int k0 = copy << (2 - copies), k1 = (copy + 1) << (2 - copies);  // its runs of 32 positions
             float m = -INFINITY, l = 0.0f;
-            const int items = d.items();
+            // Items of 128 positions (every second tile), or of 64 (both
+            // halves of every tile, so that a half's scores are made while the
+            // other's are worked on).
+            const int nt = d.t1 - d.t0, items = both ? 2 * nt : nt;
+            const int k0 = both ? 0 : copy << (2 - copies), k1 = both ? 2 : (copy + 1) << (2 - copies);  // runs of 32
 #pragma unroll 1
-            for (int w = st; w < items; w += 2) {
-                mbar_wait(&s_full[st], s_phase, abort, p.status);
-                s_phase ^= 1;
+            for (int w = both ? 0 : st; w < items; w += both ? 1 : 2) {
+                const int h = both ? w & 1 : 0;
+                const bool fresh = both ? w == 0 : w < 2;  // this stream's O holds nothing yet
+                mbar_wait(&s_full[2 * st + h], (s_phase >> h) & 1, abort, p.status);
+                s_phase ^= 1u << h;
                 tc_fence_after();
                 if (warp_on) {
-                    const int pos = (d.t0 + (both ? w >> 1 : w)) * TILE;
-                    if (pos + TILE > d.ctx) {  // drafted positions, or the end: hidden scores become -inf
+                    const int pos = both ? d.t0 * TILE + 64 * w : (d.t0 + w) * TILE;
+                    const uint32_t ts = tmem + lanes + st * TILE + 64 * h;
+                    if (pos + 32 * k1 > d.ctx) {  // drafted positions, or the end: hidden scores become -inf
 #pragma unroll 1
                         for (int k = 2 * k0; k < 2 * k1; ++k) {
                             uint32_t x[16];
@@ -699,7 +735,13 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                         const float corr = !raise ? 1.0f : m == -INFINITY ? 0.0f : exp2_approx((m - top) * sc);
                         if (raise) m = top;
                         l *= corr;
-                        if (w >= 2) {  // this stream's O holds something
+                        if (!fresh) {
+                            // The last item's product has to be in O; a whole
+                            // tile's scores come after it anyway.
+                            if (both) {
+                                mbar_wait(&pv_done[st], (products - 1) & 1, abort, p.status);
+                                tc_fence_after();
+                            }
 #pragma unroll 1
                             for (int c = 0; c < HD; c += 16) {
                                 uint32_t o[16];
@@ -727,18 +769,14 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                     };
 #pragma unroll 1
                     for (int k = k0; k < k1; k += 2) {
-                        if (!single) tmem_ld_32x32b_x32(ts + 32 * (k + 1), v0);
+                        const bool again = k1 - k0 == 4;  // two runs are both in registers
+                        if (again) tmem_ld_32x32b_x32(ts + 32 * (k + 1), v0);
                         weigh(v1, k);
                         if (!single) {
-                            arrive(v0);
+                            if (again) arrive(v0);
                             if (k + 2 < k1) tmem_ld_32x32b_x32(ts + 32 * (k + 2), v1);
                             weigh(v0, k + 1);
-                            if (k + 2 < k1) {
-                                tmem_wait_st();  // the first half of the row's probabilities
-                                tc_fence_before();
-                                mbar_arrive(&p_half[st]);
-                                arrive(v1);
-                            }
+                            if (k + 2 < k1) arrive(v1);
                         }
                     }
                     if (copies) {  // the other copies' positions
@@ -751,8 +789,9 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                     tmem_wait_st();
                 }
                 tc_fence_before();
-                if (!copies && !warp_on) mbar_arrive(&p_half[st]);
-                mbar_arrive(&p_full[st]);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[2 * st + h]);
+                if (both) ++products;
             }
             mbar_wait(unit_done, u_phase, abort, p.status);
             u_phase ^= 1;
