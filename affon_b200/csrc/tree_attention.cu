@@ -293,10 +293,9 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
     char *ring = qbuf + 2 * C::TILE_BYTES;
     uint64_t *full = reinterpret_cast<uint64_t *>(ring + C::STAGES * C::TILE_BYTES);
     uint64_t *empty = full + C::STAGES;
-    uint64_t *s_full = empty + C::STAGES;  // [2 streams][2 halves] scores are in tensor memory
-    uint64_t *p_full = s_full + 4;         // [2][2] probabilities are
-    uint64_t *pv_done = p_full + 4;        // [2] a half's product is in O
-    uint64_t *q_full = pv_done + 2;        // [2] query buffers
+    uint64_t *s_full = empty + C::STAGES;  // [2] scores of a stream are in tensor memory
+    uint64_t *p_full = s_full + 2;         // [2] probabilities of a stream are
+    uint64_t *q_full = p_full + 2;         // [2] query buffers
     uint64_t *q_empty = q_full + 2;
     uint64_t *d_full = q_empty + 2;        // [PIECES] the queue
     uint64_t *d_empty = d_full + PIECES;
@@ -317,11 +316,8 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
             mbar_init(&empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&s_full[2 * i], 1);
-            mbar_init(&s_full[2 * i + 1], 1);
-            mbar_init(&p_full[2 * i], SOFTMAX_WARPS / 2);
-            mbar_init(&p_full[2 * i + 1], SOFTMAX_WARPS / 2);
-            mbar_init(&pv_done[i], 1);
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], SOFTMAX_WARPS / 2);
             mbar_init(&q_full[i], 1);
             mbar_init(&q_empty[i], SOFTMAX_WARPS);
         }
@@ -527,12 +523,11 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
     } else if (warp == MMA) {  // ---------------------------------------------------- tensor cores
         // A negative scale negates the queries, so the running maximum can
         // work on the scores as they come.
-        const uint32_t negate = p.a.scale < 0.0f ? kUmmaNegateA : 0u;
-        const uint32_t idesc_s = umma_idesc_bf16(128, TILE) | negate, idesc_h = umma_idesc_bf16(128, TILE / 2) | negate;
+        const uint32_t idesc_s = umma_idesc_bf16(128, TILE) | (p.a.scale < 0.0f ? kUmmaNegateA : 0u);
         const uint32_t idesc_o = umma_idesc_bf16(128, HD) | kUmmaTransposeB;
         const uint32_t q_lo = umma_lo(smem_u32(qbuf), 16), k_lo = umma_lo(smem_u32(ring), 16);
         const uint32_t v_lo = umma_lo(smem_u32(ring), HALF_BYTES);
-        constexpr uint32_t TILE_LO = C::TILE_BYTES >> 4, SUB_LO = 64 * 128 >> 4;  // a tile, 64 positions of it
+        constexpr uint32_t TILE_LO = C::TILE_BYTES >> 4;
         int next = 0;  // the ring's next stage: tiles are used in the order in which they are loaded
         uint32_t next_phase = 0, p_phase = 0, pieces = 0;
         bool live = true;
@@ -551,42 +546,39 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                 if (++next == C::STAGES) next = 0, next_phase ^= 1;
                 return stage;
             };
-            auto p_ready = [&](int i) {
-                live = live && warp_wait(&p_full[i], (p_phase >> i) & 1, abort, p.status);
-                p_phase ^= 1u << i;
+            auto p_ready = [&](int st) {
+                live = live && warp_wait(&p_full[st], (p_phase >> st) & 1, abort, p.status);
+                p_phase ^= 1u << st;
                 tc_fence_after();
             };
-            // A tile's values have landed; returns the 16-position steps that hold any of its positions.
+            auto scores = [&](int st, int q, int k) {
+                umma_run_ss<HD / 16>(tmem + st * TILE, q_lo + q * TILE_LO, k_lo + k * TILE_LO, idesc_s, &s_full[st]);
+            };
+            // O += P V over the 16-position steps that hold any position of the sequence.
+            auto values = [&](int st, int v, int steps, bool accumulate) {
+                const uint32_t o = tmem + 2 * TILE + st * HD, pr = tmem + st * TILE, lo = v_lo + v * TILE_LO;
+                if (steps == 8) {
+                    umma_run_ts4(o, pr, lo, idesc_o, accumulate);
+                    umma_run_ts4(o, pr + 32, lo + 512, idesc_o, 1u);
+                } else {
+#pragma unroll 1
+                    for (int ks = 0; ks < steps; ++ks)
+                        umma_step_ts(o, pr + 8 * ks, lo + 128 * ks, idesc_o, accumulate || ks > 0);
+                }
+            };
+            // A tile's values have landed; returns their steps.
             auto enter = [&](int t, int stage) {
                 const int pos = (tile0 + t) * TILE, valid = min(TILE, len - pos);
                 if (live && pos + TILE > ctx)
                     clean_values<HD>(ring + stage * C::TILE_BYTES, max(0, ctx - pos), valid, pos - ctx, odd);
                 return (valid + 15) >> 4;
             };
-            // O += P V of 64 positions, `steps` of their 4 steps.
-            auto values = [&](int st, uint32_t p_tmem, uint32_t lo, int steps, bool accumulate) {
-                const uint32_t o = tmem + 2 * TILE + st * HD;
-                if (steps >= 4) {
-                    umma_run_ts4(o, p_tmem, lo, idesc_o, accumulate);
-                } else {
-#pragma unroll 1
-                    for (int ks = 0; ks < steps; ++ks)
-                        umma_step_ts(o, p_tmem + 8 * ks, lo + 128 * ks, idesc_o, accumulate || ks > 0);
-                }
-            };
 #pragma unroll 1
             for (int t = 0; t < (both ? 1 : 2) && t < nt; ++t) {
                 const int k = take();
                 if (!live) break;
-                const uint32_t lo = k_lo + k * TILE_LO;
-                if (both) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        umma_run_ss<HD / 16>(tmem + (i & 1) * TILE + (i >> 1) * 64, q_lo + (i & 1) * TILE_LO,
-                                             lo + (i >> 1) * SUB_LO, idesc_h, &s_full[2 * (i & 1) + (i >> 1)]);
-                } else {
-                    umma_run_ss<HD / 16>(tmem + t * TILE, q_lo + slot * TILE_LO, lo, idesc_s, &s_full[2 * t]);
-                }
+                scores(t, both ? 0 : slot, k);
+                if (both) scores(1, 1, k);
                 umma_commit_elect(&empty[k]);
             }
             if (pieces && live) live = warp_wait(o_free, (pieces - 1) & 1, abort, p.status);
@@ -597,39 +589,32 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
             for (int t = 0; t < nt && live; ++t) {
                 const int v = take();
                 const int steps = enter(t, v);
-                const uint32_t lo = v_lo + v * TILE_LO;
                 if (both) {
                     const bool more = t + 1 < nt;
-                    int k = 0;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int st = i & 1, h = i >> 1;
-                        p_ready(2 * st + h);
-                        if (!live) break;
-                        values(st, tmem + st * TILE + h * 64, lo + h * SUB_LO, steps - 4 * h, t > 0 || h > 0);
-                        umma_commit_elect(&pv_done[st]);
-                        if (more) {
-                            if (i == 0) k = take();
-                            if (!live) break;
-                            umma_run_ss<HD / 16>(tmem + st * TILE + h * 64, q_lo + st * TILE_LO,
-                                                 k_lo + k * TILE_LO + h * SUB_LO, idesc_h, &s_full[2 * st + h]);
-                        }
-                    }
+                    p_ready(0);
                     if (!live) break;
+                    values(0, v, steps, t > 0);
+                    const int k = more ? take() : 0;
+                    if (!live) break;
+                    if (more) scores(0, 0, k);
+                    p_ready(1);
+                    if (!live) break;
+                    values(1, v, steps, t > 0);
                     umma_commit_elect(&empty[v]);
-                    if (more) umma_commit_elect(&empty[k]);
+                    if (more) {
+                        scores(1, 1, k);
+                        umma_commit_elect(&empty[k]);
+                    }
                 } else {
                     const int st = t & 1;
-                    p_ready(2 * st);
+                    p_ready(st);
                     if (!live) break;
-                    values(st, tmem + st * TILE, lo, steps, t >= 2);
-                    values(st, tmem + st * TILE + 32, lo + SUB_LO, steps - 4, true);
+                    values(st, v, steps, t >= 2);
                     umma_commit_elect(&empty[v]);
                     if (t + 2 < nt) {
                         const int k = take();
                         if (!live) break;
-                        umma_run_ss<HD / 16>(tmem + st * TILE, q_lo + slot * TILE_LO, k_lo + k * TILE_LO, idesc_s,
-                                             &s_full[2 * st]);
+                        scores(st, slot, k);
                         umma_commit_elect(&empty[k]);
                     }
                 }
@@ -648,9 +633,9 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
     } else {  // ------------------------------------------------------------------------ softmax
         const int st = warp >> 2, r = tid & 127;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t to = tmem + lanes + 2 * TILE;
+        const uint32_t ts = tmem + lanes + st * TILE, to = tmem + lanes + 2 * TILE;
         const float sc = fabsf(p.a.scale) * LOG2E;
-        uint32_t s_phase = 0, u_phase = 0, products = 0;
+        uint32_t s_phase = 0, u_phase = 0;
         bool shares[2] = {false, false};
         QuerySlots slots;
         Piece d;
@@ -671,21 +656,15 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                 if (r == 0) mbar_arrive(&q_full[st]);
             }
             float m = -INFINITY, l = 0.0f;
-            // Items of 128 positions (every second tile), or of 64 (both
-            // halves of every tile, so that a half's scores are made while the
-            // other's are worked on).
-            const int nt = d.t1 - d.t0, items = both ? 2 * nt : nt;
-            const int k0 = both ? 0 : copy << (2 - copies), k1 = both ? 2 : (copy + 1) << (2 - copies);  // runs of 32
+            const int nt = d.t1 - d.t0, stride = both ? 1 : 2;
+            const int k0 = copy << (2 - copies), k1 = (copy + 1) << (2 - copies);  // this copy's runs of 32 positions
 #pragma unroll 1
-            for (int w = both ? 0 : st; w < items; w += both ? 1 : 2) {
-                const int h = both ? w & 1 : 0;
-                const bool fresh = both ? w == 0 : w < 2;  // this stream's O holds nothing yet
-                mbar_wait(&s_full[2 * st + h], (s_phase >> h) & 1, abort, p.status);
-                s_phase ^= 1u << h;
+            for (int t = both ? 0 : st; t < nt; t += stride) {
+                mbar_wait(&s_full[st], s_phase, abort, p.status);
+                s_phase ^= 1;
                 tc_fence_after();
                 if (warp_on) {
-                    const int pos = both ? d.t0 * TILE + 64 * w : (d.t0 + w) * TILE;
-                    const uint32_t ts = tmem + lanes + st * TILE + 64 * h;
+                    const int pos = (d.t0 + t) * TILE;
                     if (pos + 32 * k1 > d.ctx) {  // drafted positions, or the end: hidden scores become -inf
 #pragma unroll 1
                         for (int k = 2 * k0; k < 2 * k1; ++k) {
@@ -735,13 +714,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                         const float corr = !raise ? 1.0f : m == -INFINITY ? 0.0f : exp2_approx((m - top) * sc);
                         if (raise) m = top;
                         l *= corr;
-                        if (!fresh) {
-                            // The last item's product has to be in O; a whole
-                            // tile's scores come after it anyway.
-                            if (both) {
-                                mbar_wait(&pv_done[st], (products - 1) & 1, abort, p.status);
-                                tc_fence_after();
-                            }
+                        if (t >= stride) {  // O holds something: the scores came after the last product
 #pragma unroll 1
                             for (int c = 0; c < HD; c += 16) {
                                 uint32_t o[16];
@@ -790,8 +763,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[2 * st + h]);
-                if (both) ++products;
+                if (lane == 0) mbar_arrive(&p_full[st]);
             }
             mbar_wait(unit_done, u_phase, abort, p.status);
             u_phase ^= 1;
@@ -835,7 +807,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
             constexpr int W = HD / 4, CH = W / 8;
             const int dim0 = both ? 0 : st * (HD / 2), dim1 = both ? HD : dim0 + HD / 2;
             const int rows = both ? min(TILE, d.rows - st * TILE) : d.rows;
-            const bool pair = !both && items > 1;  // the second stream's O holds something
+            const bool pair = !both && nt > 1;  // the second stream's O holds something
             char *stage = both ? qbuf + st * C::TILE_BYTES : scratch + st * (C::TILE_BYTES / 2);
             auto cell = [&](int row, int c) {  // 16 bytes, spread over the banks
                 return reinterpret_cast<float4 *>(stage + row * (W * 4) + ((c ^ (row >> (HD == 64) & (W / 4 - 1))) << 4));
