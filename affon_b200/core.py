@@ -157,6 +157,7 @@ class Session:
             check(L.affon_b200_ctx_reserve_workspace(ctx, int(workspace_bytes)), "workspace")
         self.device = device
         self.disposed = False
+        self._bound = 0  # the stream the context was created on
         self._cache = {}
 
     # -- tensors ---------------------------------------------------------
@@ -193,9 +194,16 @@ class Session:
     def _stream(self):
         return torch.cuda.current_stream(self.torch_device).cuda_stream
 
+    def bind_stream(self):
+        """Point the context at torch's current stream of the Session's device."""
+        raw = torch._C._cuda_getCurrentRawStream(self.ordinal)
+        if raw != self._bound:
+            check(_lib.lib().affon_b200_ctx_set_stream(self._ctx, raw))
+            self._bound = raw
+
     def launch_qmm(self, desc, x, w, s, b, y, selection=None):
         L = _lib.lib()
-        check(L.affon_b200_ctx_set_stream(self._ctx, self._stream()))
+        self.bind_stream()
         sel = selection if selection is not None else None
         status = L.affon_b200_qmm_explain(self._ctx, ctypes.byref(desc), x, w, s, b, y,
                                           ctypes.byref(sel) if sel is not None else None)

@@ -51,6 +51,7 @@ import torch
 from . import _lib
 from . import tp as tpmod
 from .core import check
+from .paged import Accepted, TreePlan
 
 
 @dataclass(frozen=True)
@@ -199,7 +200,7 @@ class QuantizedDecoder:
                                 "down": down})
         self.final_norm = gamma()
         self.lm_head = shard(QuantLinear(c.vocab, c.d_model, c.bits, c.group, gen, dev), rows=[(v0, v1)])
-        kv_shape = (c.layers, batch, kv_l, capacity, c.head_dim)
+        kv_shape = self._kv_shape(kv_l)
         self.k_cache = torch.zeros(kv_shape, dtype=torch.bfloat16, device=dev)
         self.v_cache = torch.zeros(kv_shape, dtype=torch.bfloat16, device=dev)
         self.cos, self.sin = rope_tables(c, capacity, dev)
@@ -236,6 +237,9 @@ class QuantizedDecoder:
         self._build_calls()
         self.graph = None
         self._pos_host = 0   # host copy of the device position, to refuse steps beyond capacity
+
+    def _kv_shape(self, kv_heads):
+        return (self.cfg.layers, self.B, kv_heads, self.cap, self.cfg.head_dim)
 
     # -- launch descriptors --------------------------------------------------
     def _build_calls(self):
@@ -327,21 +331,27 @@ class QuantizedDecoder:
             elif kind == "allreduce":
                 self.tp.allreduce(call[1], call[2])
             elif kind == "attn":
-                kc, vc = self._kv_layer[call[1]]
-                check(L.affon_b200_decode_attention(ctx, ctypes.byref(self.attn_desc), self.qkv.data_ptr(),
-                                                    kc.data_ptr(), vc.data_ptr(), self.cos.data_ptr(),
-                                                    self.sin.data_ptr(), self.pos.data_ptr(), self.attn.data_ptr()),
-                      "decode_attention")
+                self._launch_attention(call[1])
             else:
                 _, desc, x, lin, y, fus = call
                 check(L.affon_b200_qmv_fused(ctx, ctypes.byref(desc), x, lin.w.data_ptr(), lin.s.data_ptr(),
                                              lin.b.data_ptr(), y, ctypes.byref(fus)), "qmv_fused")
             mark(ci + 2)
         if finalize or events:
-            check(L.affon_b200_argmax_finalize(ctx, self.amax.data_ptr(), self.B, self.tokens.data_ptr(),
-                                               self.history.data_ptr(), self.history.shape[0], self.pos.data_ptr(),
-                                               self.step_ctr.data_ptr()), "finalize")
+            self._launch_finalize()
             mark(len(self.calls) + 2)
+
+    def _launch_attention(self, layer):
+        kc, vc = self._kv_layer[layer]
+        check(self._L.affon_b200_decode_attention(self.ctx, ctypes.byref(self.attn_desc), self.qkv.data_ptr(),
+                                                  kc.data_ptr(), vc.data_ptr(), self.cos.data_ptr(),
+                                                  self.sin.data_ptr(), self.pos.data_ptr(), self.attn.data_ptr()),
+              "decode_attention")
+
+    def _launch_finalize(self):
+        check(self._L.affon_b200_argmax_finalize(self.ctx, self.amax.data_ptr(), self.B, self.tokens.data_ptr(),
+                                                 self.history.data_ptr(), self.history.shape[0], self.pos.data_ptr(),
+                                                 self.step_ctr.data_ptr()), "finalize")
 
     # -- public --------------------------------------------------------------
     def set_stream(self, stream):
@@ -434,9 +444,8 @@ class QuantizedDecoder:
             idx[0] += 1
             return v
         if role == "attn":
-            return lambda: check(L.affon_b200_decode_attention(
-                ctx, ctypes.byref(self.attn_desc), self.qkv.data_ptr(), *[t.data_ptr() for t in nxt(self._kv_layer)],
-                self.cos.data_ptr(), self.sin.data_ptr(), self.pos.data_ptr(), self.attn.data_ptr()))
+            layers = range(c.layers)
+            return lambda: self._launch_attention(nxt(layers))
         if role == "norm":
             gammas = [l["attn_norm"] for l in self.layers]
             return lambda: check(L.affon_b200_qmv_prep(
@@ -541,3 +550,191 @@ class QuantizedDecoder:
         c = self.cfg
         kv = 2 * self.B * self.kv_heads_local * (pos + 1) * c.head_dim * 2 * c.layers
         return weight_bytes(c) // self.world + kv
+
+
+class PagedDecoder(QuantizedDecoder):
+    """Greedy decoder over a paged KV cache, for sequences of different
+    lengths and steps that verify drafted tokens.
+
+    A step feeds up to `rows` rows (at most 32, the decode qmv's rows) that
+    belong to `seqs` sequences: `set_step` names each sequence's nodes -- its
+    last sampled token, then any drafts, as a tree of parents -- and a step
+    runs them through the model, accepts the longest drafted path that the
+    model's own choices follow, and advances every sequence by it.  Afterwards
+    `accepted` holds counts, path, next_tokens and lens (device tensors), and
+    `predicted` the model's choice after every row.  One node per sequence is
+    plain decoding; a chain of prompt tokens whose predictions are not compared
+    (`accept=False`) fills the cache.
+
+    Each sequence can hold `capacity` positions; the pool has `pages` pages of
+    `page_size` positions, handed out by `reserve` and returned by `release`.
+    The plan of a step, the rotation and append, the tree attention and the
+    acceptance are the affon_b200 paged-cache kernels; everything else is the
+    QuantizedDecoder's (with the same weights for the same seed)."""
+
+    def __init__(self, cfg, seqs, rows, device, capacity, pages, page_size=64, max_nodes=None, seed=0,
+                 workspace_bytes=None, overlap=True):
+        if not 1 <= seqs <= rows:
+            raise ValueError("a step needs a row for each of its 1 or more sequences")
+        self.seqs, self.page_size, self.pages = seqs, page_size, pages
+        self.max_nodes = min(rows, max_nodes or rows)
+        super().__init__(cfg, rows, capacity, device, seed=seed, max_steps=1, workspace_bytes=workspace_bytes,
+                         overlap=overlap)
+        dev = self.device
+        i32 = lambda *shape: torch.zeros(shape, dtype=torch.int32, device=dev)
+        per = -(-capacity // page_size)
+        self.page_table, self.ctx_lens, self.cu_nodes = i32(seqs, per), i32(seqs), i32(seqs + 1)
+        self.parents, self.predicted = i32(rows), i32(rows)
+        words = -(-self.max_nodes // 32)
+        self.plan = TreePlan(i32(rows), i32(rows), i32(rows, words))
+        self.accepted = Accepted(i32(seqs), i32(seqs, self.max_nodes), i32(seqs), self.ctx_lens)
+        self._free = list(range(pages - 1, -1, -1))
+        self._pages_of = [[] for _ in range(seqs)]
+        self._accept = True
+        c, hd = cfg, cfg.head_dim
+        st = self.k_cache.stride()
+        self._paged = _lib.PagedDesc(ctypes.sizeof(_lib.PagedDesc), seqs, rows, self.max_nodes, c.kv_heads, hd,
+                                     page_size, words, pages, st[1], st[2], st[3], per)
+        check(self._L.affon_b200_paged_validate(ctypes.byref(self._paged)), "PagedDecoder")
+        qc, kc = c.q_heads * hd, c.kv_heads * hd
+        self._append = _lib.AppendDesc(ctypes.sizeof(_lib.AppendDesc), _lib.BF16, _lib.ROPE["half"], c.q_heads, 0, qc,
+                                       qc + kc, capacity, qc + 2 * kc, qc)
+        self._tree = _lib.TreeAttnDesc(ctypes.sizeof(_lib.TreeAttnDesc), c.q_heads, 1.0 / math.sqrt(hd),
+                                       1 if c.bits == 4 else 0, qc, qc)
+        self.q = torch.zeros((rows, qc), dtype=torch.bfloat16, device=dev)
+
+    def _kv_shape(self, kv_heads):
+        return (self.cfg.layers, self.pages, kv_heads, self.page_size, self.cfg.head_dim)
+
+    def launches_per_step(self):
+        # the plan, an append before each attention, and the acceptance or (without it) the sequences' advance
+        return super().launches_per_step() + 2 + self.cfg.layers
+
+    # -- pages and steps -------------------------------------------------------
+    def reserve(self, seq, positions):
+        """Give sequence `seq` pages for at least `positions` positions."""
+        if not 0 <= positions <= self.cap:
+            raise ValueError(f"{positions} positions do not fit the capacity {self.cap}")
+        mine = self._pages_of[seq]
+        need = -(-positions // self.page_size) - len(mine)
+        if need <= 0:
+            return
+        if need > len(self._free):
+            raise ValueError(f"the pool has {len(self._free)} free pages, {need} are needed")
+        new = [self._free.pop() for _ in range(need)]
+        self.page_table[seq, len(mine):len(mine) + need] = torch.tensor(new, dtype=torch.int32, device=self.device)
+        mine += new
+
+    def release(self, seq):
+        """Return the sequence's pages; it holds nothing afterwards."""
+        self._free += reversed(self._pages_of[seq])
+        self._pages_of[seq] = []
+        self.ctx_lens[seq] = 0
+
+    def set_step(self, nodes, parents=None, tokens=None):
+        """The next steps' rows: nodes[s] nodes of sequence s, in order; parents and tokens give each row's parent
+        (within its sequence; None: every node continues the one before it) and token."""
+        nodes = [int(n) for n in nodes]
+        if len(nodes) != self.seqs or min(nodes) < 0 or max(nodes) > self.max_nodes or sum(nodes) > self.B:
+            raise ValueError(f"nodes must be {self.seqs} counts of at most {self.max_nodes}, {self.B} in all")
+        cu = [0]
+        for n in nodes:
+            cu.append(cu[-1] + n)
+        if parents is None:
+            parents = [i - 1 for n in nodes for i in range(n)]
+        host = lambda v: torch.as_tensor(v, dtype=torch.int32)
+        self.cu_nodes.copy_(host(cu))
+        self.parents[:cu[-1]] = host(parents).to(self.device)
+        if tokens is not None:
+            self.tokens[:cu[-1]] = host(tokens).to(self.device)
+
+    def _launch_step(self, finalize=True, events=None):
+        ptr = lambda t: t.data_ptr()
+        check(self._L.affon_b200_paged_plan(self.ctx, ctypes.byref(self._paged), ptr(self.cu_nodes), ptr(self.parents),
+                                            ptr(self.ctx_lens), ptr(self.page_table), ptr(self.plan.positions),
+                                            ptr(self.plan.slots), ptr(self.plan.mask)), "paged_plan")
+        super()._launch_step(finalize, events)
+
+    def _launch_attention(self, layer):
+        L, ctx, desc, p = self._L, self.ctx, ctypes.byref(self._paged), self.plan
+        kc, vc = (t.data_ptr() for t in self._kv_layer[layer])
+        check(L.affon_b200_paged_append(ctx, desc, ctypes.byref(self._append), self.qkv.data_ptr(), self.cos.data_ptr(),
+                                        self.sin.data_ptr(), p.positions.data_ptr(), p.slots.data_ptr(),
+                                        self.q.data_ptr(), kc, vc), "paged_append")
+        check(L.affon_b200_tree_attention(ctx, desc, ctypes.byref(self._tree), self.q.data_ptr(),
+                                          self.cu_nodes.data_ptr(), self.ctx_lens.data_ptr(),
+                                          self.page_table.data_ptr(), p.mask.data_ptr(), kc, vc, self.attn.data_ptr()),
+              "tree_attention")
+
+    def _launch_finalize(self):
+        L, ctx, a = self._L, self.ctx, self.accepted
+        check(L.affon_b200_argmax_finalize(ctx, self.amax.data_ptr(), self.B, self.predicted.data_ptr(), None, 0,
+                                           self.pos.data_ptr(), self.step_ctr.data_ptr()), "finalize")
+        # Without acceptance every row is taken as it is: its token is what the row before it is held to predict.
+        expected = self.predicted if self._accept else self._follow
+        check(L.affon_b200_tree_accept(ctx, ctypes.byref(self._paged), self.cfg.layers, self.k_cache.stride(0),
+                                       self.cu_nodes.data_ptr(), self.parents.data_ptr(), self.tokens.data_ptr(),
+                                       expected.data_ptr(), self.page_table.data_ptr(), self.ctx_lens.data_ptr(),
+                                       self.k_cache.data_ptr(), self.v_cache.data_ptr(), a.counts.data_ptr(),
+                                       a.path.data_ptr(), self.max_nodes, a.next_tokens.data_ptr(), a.lens.data_ptr()),
+              "tree_accept")
+
+    def _advance(self):
+        pass  # the kernels check every sequence's length against its pages
+
+    def reset(self, pos=0):
+        """Empty every sequence (their pages stay reserved)."""
+        if pos != 0:
+            raise ValueError("sequences of a paged cache start empty")
+        self.ctx_lens.zero_()
+        self._pos_host = 0
+
+    def prefill(self, prompts):
+        """Fill each sequence with its prompt (lists of tokens, one per sequence; may be empty), in steps of as many
+        rows as fit; afterwards accepted.next_tokens holds the token the model samples after a prompt's last one (for
+        the sequences whose prompt ended in the last step that fed them)."""
+        if len(prompts) != self.seqs:
+            raise ValueError(f"prefill needs {self.seqs} prompts")
+        self.reset()
+        self._follow = torch.zeros_like(self.predicted)
+        done, graph = [0] * self.seqs, self.graph
+        sampled = torch.full_like(self.accepted.next_tokens, -1)
+        for s, prompt in enumerate(prompts):
+            self.reserve(s, len(prompt))
+        self._accept, self.graph = False, None
+        try:
+            while any(d < len(p) for d, p in zip(done, prompts)):
+                room, nodes = self.B, []
+                for d, p in zip(done, prompts):
+                    nodes.append(min(self.max_nodes, room, len(p) - d))
+                    room -= nodes[-1]
+                fed = [list(p[d:d + n]) for d, p, n in zip(done, prompts, nodes)]
+                self.set_step(nodes, tokens=[t for f in fed for t in f])
+                follow = [t for f in fed for t in f[1:] + [-1] * min(1, len(f))]
+                self._follow[:len(follow)] = torch.tensor(follow, dtype=torch.int32, device=self.device)
+                self.step_eager()
+                ends = self.cu_nodes[1:] - 1
+                for s in range(self.seqs):
+                    if nodes[s] and done[s] + nodes[s] == len(prompts[s]):
+                        sampled[s] = self.predicted[ends[s]]
+                done = [d + n for d, n in zip(done, nodes)]
+        finally:
+            self._accept, self.graph = True, graph
+        self.accepted.next_tokens.copy_(sampled)
+
+    def step_bytes(self, positions):
+        """Algorithmic HBM bytes of one step with `positions` positions in every sequence: every weight once and
+        every cached key and value once."""
+        c = self.cfg
+        return weight_bytes(c) + 2 * self.seqs * c.kv_heads * (positions + 1) * c.head_dim * 2 * c.layers
+
+    def fill_kv_random(self, T, seed=0):
+        """Synthetic caches: every sequence holds T positions of N(0,1) bf16 keys and values."""
+        g = torch.Generator(device=self.device)
+        g.manual_seed(seed)
+        for s in range(self.seqs):
+            self.reserve(s, T)
+        for t in (self.k_cache, self.v_cache):
+            for li in range(t.shape[0]):
+                t[li].normal_(generator=g)
+        self.ctx_lens.fill_(T)

@@ -31,6 +31,7 @@ from . import _lib
 from .core import AffonError, check
 
 _FLOAT = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
+_BF16 = (torch.bfloat16,)
 
 
 def _check(cond, message, code="invalid_shape"):
@@ -53,6 +54,8 @@ def _tensor(session, t, name, dtypes, dim, dense=False):
 
 
 def _ints(session, t, name, shape):
+    if _dense(t, torch.int32, shape, session.torch_device):
+        return t
     _tensor(session, t, name, (torch.int32,), len(shape), dense=True)
     _check(tuple(t.shape) == shape, f"{name} must have shape {list(shape)}, not {list(t.shape)}")
     return t
@@ -63,12 +66,36 @@ def _row_stride(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _launch(session, fn, *args):
+def _dense(t, dtype, shape, device):
+    """Whether t needs no closer look (the checks of a decode step's calls are most of their host time)."""
+    return (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == device
+            and t.is_contiguous())
+
+
+def _rows_of(session, t, name, dtypes, rows, cols, more=False):
+    """A [rows, cols] tensor, dense along its rows (`more`: with further columns); returns the elements between rows."""
+    if isinstance(t, torch.Tensor) and t.dtype in dtypes and _dense(t, t.dtype, (rows, cols), session.torch_device):
+        return cols
+    _tensor(session, t, name, dtypes, 2)
+    _check(t.shape[0] == rows and (t.shape[1] == cols or more and t.shape[1] > cols),
+           f"{name} must be [{rows}, {cols}{' or more' if more else ''}], not {list(t.shape)}")
+    return _row_stride(t)
+
+
+def _ready(session):
     if session.disposed:
         raise AffonError("invalid_arg", "Session has been disposed")
-    L = _lib.lib()
-    check(L.affon_b200_ctx_set_stream(session._ctx, session._stream()))
-    check(getattr(L, fn)(session._ctx, *args))
+    session.bind_stream()
+    return _lib.lib()
+
+
+def _tables(session, cos, sin, half):
+    """Rotation tables [positions, half]; returns the positions."""
+    for t, name in ((cos, "cos"), (sin, "sin")):
+        if not (isinstance(t, torch.Tensor) and _dense(t, torch.float32, t.shape, session.torch_device) and t.dim() == 2):
+            _tensor(session, t, name, (torch.float32,), 2, dense=True)
+    _check(cos.shape == sin.shape and cos.shape[1] == half, f"cos and sin must be [positions, {half}]")
+    return cos.shape[0]
 
 
 class PagedCache:
@@ -162,7 +189,18 @@ class PagedBatch:
             cache.page_size if cache else page_size, self.mask_words, cache.pages if cache else pages, *strides, per)
         check(_lib.lib().affon_b200_paged_validate(ctypes.byref(d)), "PagedBatch")
         self._desc = ctypes.byref(d)
+        self._descs = {}
         self._step = tuple(ctypes.c_void_p(t.data_ptr()) for t in (cu_nodes, ctx_lens, page_table))
+
+    def _memo(self, desc, *fields):
+        """A reference to the call descriptor with these fields (a step's calls repeat the same few)."""
+        key = (desc,) + fields
+        ref = self._descs.get(key)
+        if ref is None:
+            if len(self._descs) >= 64:
+                self._descs.clear()
+            ref = self._descs[key] = ctypes.byref(desc(ctypes.sizeof(desc), *fields))
+        return ref
 
     def _pools(self, layer):
         _check(self.cache is not None, "the batch was made without a cache", "invalid_arg")
@@ -188,14 +226,15 @@ def plan(batch, parents=None, out=None):
     if parents is not None:
         _ints(s, parents, "parents", (batch.rows,))
     if out is None:
-        new = lambda *shape: torch.empty(shape, dtype=torch.int32, device=s.torch_device)
-        out = TreePlan(new(batch.rows), new(batch.rows), new(batch.rows, batch.mask_words))
+        new = batch.ctx_lens.new_empty
+        out = TreePlan(new(batch.rows), new(batch.rows), new((batch.rows, batch.mask_words)))
     else:
         _check_plan(batch, out)
         _check(out.mask is not None, "plan needs a mask to write", "invalid_arg")
+    L = _ready(s)
     cu, ctx, table = batch._step
-    _launch(s, "affon_b200_paged_plan", batch._desc, cu, parents.data_ptr() if parents is not None else None, ctx,
-            table, out.positions.data_ptr(), out.slots.data_ptr(), out.mask.data_ptr())
+    check(L.affon_b200_paged_plan(s._ctx, batch._desc, cu, None if parents is None else parents.data_ptr(), ctx, table,
+                                  out.positions.data_ptr(), out.slots.data_ptr(), out.mask.data_ptr()))
     return out
 
 
@@ -216,29 +255,25 @@ def append(batch, plan, qkv, q_heads, cos=None, sin=None, layer=0, rope="half", 
     written."""
     s, c = batch.session, batch.cache
     k, v = batch._pools(layer)
-    _tensor(s, qkv, "qkv", tuple(_FLOAT), 2)
-    hd, kv = c.head_dim, c.kv_heads
+    hd, kv, rows = c.head_dim, c.kv_heads, batch.rows
     _check(isinstance(q_heads, int) and q_heads >= 0, "q_heads must be a whole number")
-    _check(qkv.shape[0] == batch.rows and qkv.shape[1] >= (q_heads + 2 * kv) * hd,
-           f"qkv must have {batch.rows} rows of at least {(q_heads + 2 * kv) * hd} columns")
-    _ints(s, plan.slots, "slots", (batch.rows,))
+    ld = _rows_of(s, qkv, "qkv", _FLOAT, rows, (q_heads + 2 * kv) * hd, more=True)
+    _ints(s, plan.slots, "slots", (rows,))
     mode = _lib.ROPE.get(rope)
     _check(mode is not None, "rope must be half, interleaved or none", "invalid_arg")
+    length = 0
     if mode:
-        _ints(s, plan.positions, "positions", (batch.rows,))
-        _tensor(s, cos, "cos", (torch.float32,), 2, dense=True)
-        _tensor(s, sin, "sin", (torch.float32,), 2, dense=True)
-        _check(cos.shape == sin.shape and cos.shape[1] == hd // 2, f"cos and sin must be [positions, {hd // 2}]")
+        _ints(s, plan.positions, "positions", (rows,))
+        length = _tables(s, cos, sin, hd // 2)
     if q_out is None:
-        q_out = torch.empty((batch.rows, q_heads * hd), dtype=torch.bfloat16, device=s.torch_device)
-    else:
-        _tensor(s, q_out, "q_out", (torch.bfloat16,), 2)
-        _check(tuple(q_out.shape) == (batch.rows, q_heads * hd), f"q_out must be [{batch.rows}, {q_heads * hd}]")
-    d = _lib.AppendDesc(ctypes.sizeof(_lib.AppendDesc), _FLOAT[qkv.dtype], mode, q_heads, 0, q_heads * hd,
-                        (q_heads + kv) * hd, cos.shape[0] if mode else 0, _row_stride(qkv), _row_stride(q_out))
-    _launch(s, "affon_b200_paged_append", batch._desc, ctypes.byref(d), qkv.data_ptr(),
-            cos.data_ptr() if mode else None, sin.data_ptr() if mode else None,
-            plan.positions.data_ptr() if mode else None, plan.slots.data_ptr(), q_out.data_ptr(), k, v)
+        q_out = torch.empty((rows, q_heads * hd), dtype=torch.bfloat16, device=s.torch_device)
+    ld_q = _rows_of(s, q_out, "q_out", _BF16, rows, q_heads * hd)
+    d = batch._memo(_lib.AppendDesc, _FLOAT[qkv.dtype], mode, q_heads, 0, q_heads * hd, (q_heads + kv) * hd, length, ld,
+                    ld_q)
+    L = _ready(s)
+    check(L.affon_b200_paged_append(s._ctx, batch._desc, d, qkv.data_ptr(), cos.data_ptr() if mode else None,
+                                    sin.data_ptr() if mode else None, plan.positions.data_ptr() if mode else None,
+                                    plan.slots.data_ptr(), q_out.data_ptr(), k, v))
     return q_out
 
 
@@ -250,23 +285,21 @@ def tree_attention(batch, plan, q, q_heads, layer=0, scale=None, out=None, pair_
     head_dim**-0.5.  Padding rows of `out` are not written.  pair_order writes the 4-bit decode qmv's column order."""
     s, c = batch.session, batch.cache
     k, v = batch._pools(layer)
+    _check(isinstance(q_heads, int) and q_heads > 0, "q_heads must be a positive whole number")
     cols = q_heads * c.head_dim
-    _tensor(s, q, "q", (torch.bfloat16,), 2)
-    _check(tuple(q.shape) == (batch.rows, cols), f"q must be [{batch.rows}, {cols}], not {list(q.shape)}")
+    ld_q = _rows_of(s, q, "q", _BF16, batch.rows, cols)
     mask = plan.mask if plan is not None else None
     if mask is not None:
         _ints(s, mask, "mask", (batch.rows, batch.mask_words))
     if out is None:
         out = torch.empty((batch.rows, cols), dtype=torch.bfloat16, device=s.torch_device)
-    else:
-        _tensor(s, out, "out", (torch.bfloat16,), 2)
-        _check(tuple(out.shape) == (batch.rows, cols), f"out must be [{batch.rows}, {cols}]")
-    d = _lib.TreeAttnDesc(ctypes.sizeof(_lib.TreeAttnDesc), q_heads,
-                          c.head_dim ** -0.5 if scale is None else scale, 1 if pair_order else 0, _row_stride(q),
-                          _row_stride(out))
+    ld_out = _rows_of(s, out, "out", _BF16, batch.rows, cols)
+    d = batch._memo(_lib.TreeAttnDesc, q_heads, c.head_dim ** -0.5 if scale is None else float(scale),
+                    1 if pair_order else 0, ld_q, ld_out)
+    L = _ready(s)
     cu, ctx, table = batch._step
-    _launch(s, "affon_b200_tree_attention", batch._desc, ctypes.byref(d), q.data_ptr(), cu, ctx, table,
-            mask.data_ptr() if mask is not None else None, k, v, out.data_ptr())
+    check(L.affon_b200_tree_attention(s._ctx, batch._desc, d, q.data_ptr(), cu, ctx, table,
+                                      None if mask is None else mask.data_ptr(), k, v, out.data_ptr()))
     return out
 
 
@@ -295,17 +328,18 @@ def tree_accept(batch, parents, tokens, predicted, out=None):
     _ints(s, tokens, "tokens", (batch.rows,))
     _ints(s, predicted, "predicted", (batch.rows,))
     if out is None:
-        new = lambda *shape: torch.empty(shape, dtype=torch.int32, device=s.torch_device)
-        out = Accepted(new(batch.seqs), new(batch.seqs, batch.max_nodes), new(batch.seqs), batch.ctx_lens.clone())
+        new, seqs = batch.ctx_lens.new_empty, batch.seqs
+        out = Accepted(new(seqs), new((seqs, batch.max_nodes)), new(seqs), new(seqs))
     else:
         _ints(s, out.counts, "counts", (batch.seqs,))
         _ints(s, out.path, "path", (batch.seqs, batch.max_nodes))
         _ints(s, out.next_tokens, "next_tokens", (batch.seqs,))
         _ints(s, out.lens, "lens", (batch.seqs,))
+    L = _ready(s)
     cu, ctx, table = batch._step
     k, v = c.layer(0)
-    _launch(s, "affon_b200_tree_accept", batch._desc, c.layers, c.layer_stride, cu,
-            parents.data_ptr() if parents is not None else None, tokens.data_ptr(), predicted.data_ptr(), table, ctx, k,
-            v, out.counts.data_ptr(), out.path.data_ptr(), batch.max_nodes, out.next_tokens.data_ptr(),
-            out.lens.data_ptr())
+    check(L.affon_b200_tree_accept(s._ctx, batch._desc, c.layers, c.layer_stride, cu,
+                                   None if parents is None else parents.data_ptr(), tokens.data_ptr(),
+                                   predicted.data_ptr(), table, ctx, k, v, out.counts.data_ptr(), out.path.data_ptr(),
+                                   batch.max_nodes, out.next_tokens.data_ptr(), out.lens.data_ptr()))
     return out

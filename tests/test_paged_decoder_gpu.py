@@ -1,0 +1,201 @@
+"""The decoder over a paged cache: plain steps against the contiguous-cache
+decoder of the same weights, drafted trees against a float32 restatement of
+every node's path, and the graph-captured step."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import paged_ref as ref
+from affon_b200.core import AffonError
+from affon_b200.decoder import LlamaConfig, PagedDecoder, QuantizedDecoder
+from test_decoder_gpu import bf16, normed_proj, rope
+
+pytestmark = pytest.mark.gpu
+
+SMALL = LlamaConfig(layers=2, d_model=512, q_heads=4, kv_heads=1, head_dim=128, ffn=1024, vocab=1000)
+SMALL_G8 = LlamaConfig(layers=2, d_model=1024, q_heads=16, kv_heads=2, head_dim=128, ffn=2048, vocab=1000)
+SMALL_8BIT = LlamaConfig(layers=2, d_model=512, q_heads=8, kv_heads=2, head_dim=128, ffn=1536, vocab=1000, bits=8)
+
+
+def cached(dec, layer, seq, length):
+    """Keys and values [kv_heads, length, hd] of a sequence, float32."""
+    at = torch.arange(length, device=dec.device)
+    pages = dec.page_table[seq].long()[at // dec.page_size]
+    take = lambda pool: pool[layer][pages, :, at % dec.page_size].float().transpose(0, 1)
+    return take(dec.k_cache), take(dec.v_cache)
+
+
+def ref_tree(dec, seq, ctx, parents, tokens):
+    """float32 residual rows, logits and bf16-rounded keys/values of a tree over a sequence's first ctx positions."""
+    c = dec.cfg
+    G, hd, n = c.q_heads // c.kv_heads, c.head_dim, len(tokens)
+    seen = torch.from_numpy(ref.ancestors(parents)).to(dec.device)
+    pos = ctx + seen.sum(-1) - 1
+    cos, sin = dec.cos[pos][:, None], dec.sin[pos][:, None]
+    h = dec.embed[torch.as_tensor(tokens, device=dec.device).long()].float()
+    kept = []
+    for li, lay in enumerate(dec.layers):
+        qkv = bf16(normed_proj(h, lay["attn_norm"], lay["qkv"], c.eps))
+        q = qkv[:, :c.q_heads * hd].reshape(n, c.q_heads, hd)
+        k = qkv[:, c.q_heads * hd:(c.q_heads + c.kv_heads) * hd].reshape(n, c.kv_heads, hd)
+        v = qkv[:, (c.q_heads + c.kv_heads) * hd:].reshape(n, c.kv_heads, hd)
+        q, k = bf16(rope(q, cos, sin)), bf16(rope(k, cos, sin))
+        kept.append((k, v))
+        pk, pv = cached(dec, li, seq, ctx)
+        keys = torch.cat([pk, k.transpose(0, 1)], 1).repeat_interleave(G, 0)
+        vals = torch.cat([pv, v.transpose(0, 1)], 1).repeat_interleave(G, 0)
+        z = torch.einsum("nhd,htd->nht", q, keys) / math.sqrt(hd)
+        z[:, :, ctx:] = z[:, :, ctx:].masked_fill(~seen[:, None, :], -math.inf)
+        attn = bf16(torch.einsum("nht,htd->nhd", torch.softmax(z, -1), vals).reshape(n, -1))
+        h = h + attn @ lay["o"].dequantized().T
+        gu = normed_proj(h, lay["ffn_norm"], lay["gate_up"], c.eps).reshape(n, -1, 2, 8)
+        act = bf16(torch.nn.functional.silu(gu[:, :, 0].reshape(n, -1)) * gu[:, :, 1].reshape(n, -1))
+        h = h + act @ lay["down"].dequantized().T
+    return h, normed_proj(h, dec.final_norm, dec.lm_head, c.eps), kept
+
+
+def clear(logits):
+    top = torch.topk(logits, 2, dim=-1)
+    return (top.values[:, 0] - top.values[:, 1]) > 2e-2 * top.values[:, 0].abs().clamp(min=1), top.indices[:, 0]
+
+
+@pytest.mark.parametrize("cfg,rows,nodes,page", [(SMALL, 16, [5, 8, 1], 16), (SMALL_G8, 32, [12, 0, 20], 32),
+                                                 (SMALL_8BIT, 8, [3, 4], 64)], ids=["4q", "8q-empty", "8bit"])
+def test_drafted_step_matches_float32_reference(cfg, rows, nodes, page):
+    seqs = len(nodes)
+    rng = np.random.default_rng(rows)
+    d = PagedDecoder(cfg, seqs, rows, "cuda:0", capacity=192, pages=seqs * 192 // page, page_size=page, seed=2)
+    try:
+        lens = [37, 0, 90][:seqs]
+        d.prefill([rng.integers(0, cfg.vocab, size=n).tolist() for n in lens])
+        d.synchronize()
+        assert d.ctx_lens.tolist() == lens
+        parents = [ref.random_forest(n, rng) for n in nodes]
+        tokens = [rng.integers(0, cfg.vocab, size=n) for n in nodes]
+        want = [ref_tree(d, s, lens[s], parents[s], tokens[s]) if nodes[s] else None for s in range(seqs)]
+        for s in range(seqs):
+            # some drafts right: a child of the root is what the reference predicts there
+            ok, best = clear(want[s][1]) if nodes[s] > 1 else (torch.zeros(1, dtype=torch.bool), None)
+            kids = [j for j in range(nodes[s]) if parents[s][j] == 0]
+            if ok[0] and kids:
+                tokens[s][kids[-1]] = int(best[0])
+                want[s] = ref_tree(d, s, lens[s], parents[s], tokens[s])
+        for s in range(seqs):
+            d.reserve(s, lens[s] + nodes[s])
+        d.set_step(nodes, np.concatenate(parents), np.concatenate(tokens))
+        d.step_eager()
+        d.synchronize()
+        predicted, at = d.predicted.cpu().numpy(), 0
+        for s, n in enumerate(nodes):
+            if n == 0:
+                assert int(d.accepted.counts[s]) == 0 and int(d.ctx_lens[s]) == lens[s]
+                continue
+            h, logits, kept = want[s]
+            got = d.h[at:at + n]
+            assert float((got - h).abs().max()) <= 2e-2 * float(h.abs().max())
+            ok, best = clear(logits)
+            assert torch.equal(torch.from_numpy(predicted[at:at + n]).to(best.device)[ok].long(), best[ok])
+            step = ref.Step([lens[s]], [n], page, parents=[parents[s]])
+            counts, path, nxt, new = ref.accept(step, tokens[s], predicted[at:at + n])
+            assert d.accepted.counts[s] == counts[0] and d.ctx_lens[s] == new[0]
+            assert d.accepted.path[s, :n].tolist() == path[0].tolist() and int(d.accepted.next_tokens[s]) == nxt[0]
+            line = path[0][:counts[0]].tolist()
+            for li in range(cfg.layers):
+                k, v = cached(d, li, s, int(new[0]))
+                for pool, exact in ((k, kept[li][0]), (v, kept[li][1])):
+                    rows_ = exact[line].transpose(0, 1)
+                    assert float((pool[:, lens[s]:] - rows_).abs().max()) <= 2e-2 * max(1.0, float(rows_.abs().max()))
+            at += n
+    finally:
+        d.close()
+
+
+def test_plain_steps_fill_the_first_layer_like_the_contiguous_decoder():
+    """Same weights, the same tokens at the same positions: the first layer's keys and values come from the same
+    projection bits, so values are equal and keys (each a rotation in f32 rounded once to bf16: half a step, 2^-8
+    relative, and 2^-22 of the rotated pair's magnitudes) differ by at most two such errors.  Deeper layers differ by
+    the two attentions' roundings and are compared with a float32 restatement above."""
+    B, T = 4, 21
+    gen = torch.Generator().manual_seed(3)
+    prompt = torch.randint(0, SMALL.vocab, (T, B), generator=gen)
+    a = QuantizedDecoder(SMALL, batch=B, capacity=64, device="cuda:0", seed=7, max_steps=16)
+    b = PagedDecoder(SMALL, B, B, "cuda:0", capacity=64, pages=2 * B, page_size=32, seed=7)
+    try:
+        a.prefill(prompt)
+        b.prefill([prompt[:, s].tolist() for s in range(B)])
+        for step in range(6):
+            toks = torch.randint(0, SMALL.vocab, (B,), generator=gen, dtype=torch.int32)
+            a.tokens.copy_(toks)
+            for s in range(B):
+                b.reserve(s, T + step + 1)
+            b.set_step([1] * B, tokens=toks.tolist())
+            a.step_eager()
+            b.step_eager()
+        a.synchronize()
+        b.synchronize()
+        assert b.ctx_lens.tolist() == [T + 6] * B and int(a.pos) == T + 6
+        for s in range(B):
+            k, v = cached(b, 0, s, T + 6)
+            ka, va = (t[0][s, :, :T + 6].float() for t in (a.k_cache, a.v_cache))
+            assert torch.equal(v, va)
+            pair = ka.abs() + ka.roll(64, -1).abs()
+            assert ((k - ka).abs() <= 2 * (2.0 ** -8 * ka.abs() * 1.01 + 2.0 ** -21 * pair)).all()
+    finally:
+        a.close()
+        b.close()
+
+
+@pytest.mark.parametrize("overlap", [False, True])
+def test_captured_steps_equal_eager_ones(overlap):
+    outs = []
+    for captured in (False, True):
+        d = PagedDecoder(SMALL, 3, 12, "cuda:0", capacity=128, pages=24, page_size=16, seed=5, overlap=overlap)
+        try:
+            rng = np.random.default_rng(1)
+            d.prefill([rng.integers(0, SMALL.vocab, size=n).tolist() for n in (9, 30, 2)])
+            for s in range(3):
+                d.reserve(s, 100)
+            if captured:
+                d.set_step([4, 4, 4], tokens=[0] * 12)
+                d.capture()
+            seen = []
+            for _ in range(4):
+                par = np.concatenate([ref.random_forest(4, rng) for _ in range(3)])
+                d.set_step([4, 4, 4], par, rng.integers(0, SMALL.vocab, size=12))
+                d.replay() if captured else d.step_eager()
+                d.synchronize()
+                seen += [d.predicted.clone(), d.accepted.counts.clone(), d.ctx_lens.clone(), d.h.clone()]
+            outs.append(seen + [d.k_cache.clone(), d.v_cache.clone()])
+        finally:
+            d.close()
+    for x, y in zip(*outs):
+        assert torch.equal(x, y)
+
+
+def test_pages_are_shared_out_and_overruns_reported():
+    d = PagedDecoder(SMALL, 2, 4, "cuda:0", capacity=64, pages=3, page_size=16, seed=5)
+    try:
+        d.reserve(0, 30)
+        with pytest.raises(ValueError):
+            d.reserve(1, 30)                     # one page is left
+        with pytest.raises(ValueError):
+            d.reserve(1, 65)
+        with pytest.raises(ValueError):
+            d.set_step([3, 2])
+        d.release(0)
+        d.reserve(1, 48)
+        d.prefill([[], list(range(48))])
+        d.synchronize()
+        assert d.ctx_lens.tolist() == [0, 48]
+        k0 = d.k_cache.clone()
+        d.ctx_lens[1] = 62                       # three more nodes pass the page table's end
+        d.set_step([0, 3], tokens=[1, 2, 3])
+        d.step_eager()
+        with pytest.raises(AffonError) as err:
+            d.synchronize()
+        assert err.value.code == "invalid_arg"
+        assert torch.equal(d.k_cache, k0) and int(d.ctx_lens[1]) == 62
+    finally:
+        d.close()
