@@ -114,16 +114,18 @@ struct Piece {
 
 // Which of the two query buffers a piece uses and how often each was used.
 struct QuerySlots {
-    unsigned used[2] = {0u, 0u};
+    unsigned uses0 = 0u, uses1 = 0u;
     int next = 0;
     __device__ __forceinline__ int take(bool both) {
         const int s = both ? 0 : next;
         next = both ? 0 : next ^ 1;
-        ++used[s];
-        if (both) ++used[1];
+        uses0 += s == 0;
+        uses1 += both || s == 1;
         return s;
     }
-    __device__ __forceinline__ uint32_t parity(int slot) const { return (used[slot] - 1) & 1; }  // of its current use
+    __device__ __forceinline__ uint32_t parity(int slot) const {  // of its current use
+        return ((slot ? uses1 : uses0) - 1) & 1;
+    }
 };
 
 // 32 visibility bits of a row, for drafted nodes j0 .. j0+31 (cached
@@ -636,7 +638,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
         const uint32_t ts = tmem + lanes + st * TILE, to = tmem + lanes + 2 * TILE;
         const float sc = fabsf(p.a.scale) * LOG2E;
         uint32_t s_phase = 0, u_phase = 0;
-        bool shares[2] = {false, false};
+        bool shares_end = false, shares_start = false;  // units that other CTAs have a part of
         QuerySlots slots;
         Piece d;
         while (next_piece(d)) {
@@ -856,8 +858,12 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                 }
                 named_bar_sync(2 + st, 128);
             }
-            if (__any_sync(0xffffffffu, odd[lane & 7] != 0u) && mine && copy == 0)
-                add_odd_values(p, d, mask, odd, dim0, dim1, whole ? nullptr : rec + rr * HD, out_row<HD>(p, d, rr));
+            if (__any_sync(0xffffffffu, odd[lane & 7] != 0u) && mine && copy == 0) {
+                // Copies, so that what the call takes by address stays in registers elsewhere.
+                const Piece piece = d;
+                const RowMask seen = mask;
+                add_odd_values(p, piece, seen, odd, dim0, dim1, whole ? nullptr : rec + rr * HD, out_row<HD>(p, d, rr));
+            }
             if (!whole && mine && copy == 0 && dim0 == 0) {
                 rec[ROWS * HD + rr] = top;
                 rec[ROWS * HD + ROWS + rr] = lsum;
@@ -870,7 +876,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                 if (both) mbar_arrive(&q_empty[1]);
             }
             if (!whole) {
-                shares[d.t0 == 0] = true;
+                (d.t0 == 0 ? shares_start : shares_end) = true;
                 if (tid == 0) shared_units[d.t0 == 0] = d;
                 named_bar_sync(1, SOFTMAX_THREADS);
                 if (tid == 0) {  // the barrier's order and this fence publish all threads' stores
@@ -883,7 +889,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
         // takes 8 dims of a row and a part of the unit's pieces.
 #pragma unroll 1
         for (int which = 0; which < 2; ++which) {
-            if (!shares[which]) continue;
+            if (!(which ? shares_start : shares_end)) continue;
             const Piece u = shared_units[which];
             const int owner0 = division->owner(u.start), k = division->owner(u.start + u.nt - 1) - owner0 + 1;
             const int me = blockIdx.x - owner0;
