@@ -92,82 +92,125 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(PagedShape s, PagedS
 }
 
 // ----------------------------------------------------------------- append
-// A thread rotates or copies 16 dims of one head of one row: two runs of 8
-// (d and d + head_dim/2) or one of 16 (interleaved pairs, values).
+// A thread takes 16 dims of up to HEADS heads of one row, in two runs of 8 (d
+// and d + head_dim/2, or 16 in a row for interleaved pairs and values): the
+// row's 16 table values are loaded once for all of them, and all loads are
+// issued before the first is used.  Bound by HBM where there are many rows:
+// 13,921 rows of 8 + 8 + 32 heads of 128 (349 MB) take 59 us (5.9 TB/s,
+// 0.90 of the copy rate; one head a thread, which reads the tables again for
+// every head, took 69).
+constexpr int APPEND_HEADS = 4, APPEND_THREADS = 128;
+
 template <bool F32>
-__device__ __forceinline__ void load8(const void *base, int64_t at, float (&x)[8]) {
-    if (F32) {
-        const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(base) + at);
-        const float4 a = p[0], b = p[1];
-        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-    } else {
-        const uint4 a = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(base) + at);
-        const uint32_t u[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[2 * i] = __uint_as_float(u[i] << 16);
-            x[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+struct Run8 {
+    uint4 a, b;  // b: f32 only
+    __device__ __forceinline__ void load(const void *base, int64_t at) {
+        if (F32) {
+            const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const float *>(base) + at);
+            a = __ldg(p), b = __ldg(p + 1);
+        } else {
+            a = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(base) + at));
         }
     }
-}
+    __device__ __forceinline__ void get(float (&x)[8]) const {
+        const uint32_t u[4] = {a.x, a.y, a.z, a.w}, w[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (F32) {
+                x[i] = __uint_as_float(u[i]);
+                x[4 + i] = __uint_as_float(w[i]);
+            } else {
+                x[2 * i] = __uint_as_float(u[i] << 16);
+                x[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+            }
+        }
+    }
+};
 __device__ __forceinline__ void store8(uint16_t *dst, const float (&x)[8]) {
     *reinterpret_cast<uint4 *>(dst) = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]),
                                                  pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
 }
 
 template <bool F32>
-__global__ void append_kernel(PagedShape s, AppendArgs a, unsigned *status) {
+__global__ void __launch_bounds__(APPEND_THREADS) append_kernel(PagedShape s, AppendArgs a, unsigned per_row,
+                                                                unsigned *status) {
     pdl_launch_dependents();
     pdl_wait();
-    const int chunks = s.head_dim >> 4, heads = a.q_heads + 2 * s.kv_heads;
-    const int item = blockIdx.y * blockDim.x + threadIdx.x;
-    const int64_t row = blockIdx.x;
-    if (item >= heads * chunks) return;
-    const int head = item / chunks, chunk = item % chunks, half = s.head_dim >> 1;
+    const int chunks = s.head_dim >> 4, heads = a.q_heads + 2 * s.kv_heads, half = s.head_dim >> 1;
+    const int64_t item = static_cast<int64_t>(blockIdx.x) * APPEND_THREADS + threadIdx.x;
+    // per_row items a row; a block's items start in one row and reach into at most APPEND_THREADS more
+    const int64_t row0 = gridDim.x < 1u << 24 ? blockIdx.x * APPEND_THREADS / per_row
+                                              : static_cast<int64_t>(blockIdx.x) * APPEND_THREADS / per_row;
+    const unsigned within = static_cast<unsigned>(item - row0 * per_row);
+    const int64_t row = row0 + within / per_row;
+    if (row >= s.rows) return;
+    const int rest = within % per_row, chunk = rest % chunks, head0 = rest / chunks * APPEND_HEADS;
     const int slot = a.slots[row];
     if (slot == -1) return;
     const int pos = a.rope ? a.positions[row] : 0;
     if (slot < 0 || (slot >> s.page_shift) >= s.pages || (a.rope && (pos < 0 || pos >= a.table_rows))) {
-        if (item == 0) atomicExch(status, static_cast<unsigned>(DEV_BOUNDS));
+        if (rest == 0) atomicExch(status, static_cast<unsigned>(DEV_BOUNDS));
         return;
+    }
+    const bool half_pairs = a.rope == AFFON_B200_ROPE_HALF;
+    Run8<F32> x0[APPEND_HEADS], x1[APPEND_HEADS];
+#pragma unroll
+    for (int i = 0; i < APPEND_HEADS; ++i) {
+        const int head = head0 + i;
+        if (head >= heads) break;
+        const bool is_v = head >= a.q_heads + s.kv_heads;
+        const int col = head < a.q_heads ? a.q_off + head * s.head_dim
+                        : is_v           ? a.v_off + (head - a.q_heads - s.kv_heads) * s.head_dim
+                                         : a.k_off + (head - a.q_heads) * s.head_dim;
+        const bool apart = half_pairs && !is_v;
+        const int d0 = apart ? chunk * 8 : chunk * 16;
+        x0[i].load(a.qkv, row * a.ld_qkv + col + d0);
+        x1[i].load(a.qkv, row * a.ld_qkv + col + (apart ? d0 + half : d0 + 8));
+    }
+    float c[8], sn[8];
+    if (a.rope && head0 < a.q_heads + s.kv_heads) {
+        Run8<true> t0, t1;
+        t0.load(a.cos_t, static_cast<int64_t>(pos) * half + chunk * 8);
+        t1.load(a.sin_t, static_cast<int64_t>(pos) * half + chunk * 8);
+        t0.get(c), t1.get(sn);
     }
     const int64_t place = (slot >> s.page_shift) * s.page_stride +
                           static_cast<int64_t>(slot & ((1 << s.page_shift) - 1)) * s.token_stride;
-    const bool is_q = head < a.q_heads, is_v = head >= a.q_heads + s.kv_heads;
-    const int kv = is_q ? 0 : is_v ? head - a.q_heads - s.kv_heads : head - a.q_heads;
-    const int col = is_q ? a.q_off + head * s.head_dim : (is_v ? a.v_off : a.k_off) + kv * s.head_dim;
-    uint16_t *dst = is_q ? a.q_out + row * a.ld_q + static_cast<int64_t>(head) * s.head_dim
-                         : (is_v ? a.v_cache : a.k_cache) + place + kv * s.head_stride;
-    const bool apart = a.rope == AFFON_B200_ROPE_HALF && !is_v;
-    const int d0 = apart ? chunk * 8 : chunk * 16, d1 = apart ? d0 + half : d0 + 8;
-    float x[8], y[8];
-    load8<F32>(a.qkv, row * a.ld_qkv + col + d0, x);
-    load8<F32>(a.qkv, row * a.ld_qkv + col + d1, y);
-    if (a.rope && !is_v) {
-        float c[8], sn[8];
-        load8<true>(a.cos_t, static_cast<int64_t>(pos) * half + chunk * 8, c);
-        load8<true>(a.sin_t, static_cast<int64_t>(pos) * half + chunk * 8, sn);
-        if (apart) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float p = x[i], q = y[i];
-                x[i] = p * c[i] - q * sn[i];
-                y[i] = q * c[i] + p * sn[i];
-            }
-        } else {
+    for (int i = 0; i < APPEND_HEADS; ++i) {
+        const int head = head0 + i;
+        if (head >= heads) break;
+        const bool is_q = head < a.q_heads, is_v = head >= a.q_heads + s.kv_heads;
+        const int kv = is_q ? 0 : is_v ? head - a.q_heads - s.kv_heads : head - a.q_heads;
+        uint16_t *dst = is_q ? a.q_out + row * a.ld_q + static_cast<int64_t>(head) * s.head_dim
+                             : (is_v ? a.v_cache : a.k_cache) + place + kv * s.head_stride;
+        const bool apart = half_pairs && !is_v;
+        const int d0 = apart ? chunk * 8 : chunk * 16, d1 = apart ? d0 + half : d0 + 8;
+        float x[8], y[8];
+        x0[i].get(x), x1[i].get(y);
+        if (a.rope && !is_v) {
+            if (apart) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float p = x[2 * i], q = x[2 * i + 1];
-                x[2 * i] = p * c[i] - q * sn[i];
-                x[2 * i + 1] = q * c[i] + p * sn[i];
-                p = y[2 * i], q = y[2 * i + 1];
-                y[2 * i] = p * c[4 + i] - q * sn[4 + i];
-                y[2 * i + 1] = q * c[4 + i] + p * sn[4 + i];
+                for (int e = 0; e < 8; ++e) {
+                    const float p = x[e], q = y[e];
+                    x[e] = p * c[e] - q * sn[e];
+                    y[e] = q * c[e] + p * sn[e];
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float p = x[2 * e], q = x[2 * e + 1];
+                    x[2 * e] = p * c[e] - q * sn[e];
+                    x[2 * e + 1] = q * c[e] + p * sn[e];
+                    p = y[2 * e], q = y[2 * e + 1];
+                    y[2 * e] = p * c[4 + e] - q * sn[4 + e];
+                    y[2 * e + 1] = q * c[4 + e] + p * sn[4 + e];
+                }
             }
         }
+        store8(dst + d0, x);
+        store8(dst + d1, y);
     }
-    store8(dst + d0, x);
-    store8(dst + d1, y);
 }
 
 // ----------------------------------------------------------------- accept
@@ -293,11 +336,14 @@ cudaError_t launch_paged_plan(const PagedShape &s, const PagedStep &t, int *posi
 
 cudaError_t launch_paged_append(const PagedShape &s, const AppendArgs &a, void *workspace, cudaStream_t stream,
                                 bool pdl) {
-    const int items = (a.q_heads + 2 * s.kv_heads) * (s.head_dim >> 4);
-    const dim3 grid(s.rows, (items + 127) / 128);
-    cudaError_t e = a.x_f32 ? launch_ex(paged::append_kernel<true>, grid, dim3(128), 0, stream, false, pdl, s, a,
+    const unsigned per_row = (a.q_heads + 2 * s.kv_heads + paged::APPEND_HEADS - 1) / paged::APPEND_HEADS *
+                             (s.head_dim >> 4);
+    const int64_t blocks = (static_cast<int64_t>(s.rows) * per_row + paged::APPEND_THREADS - 1) / paged::APPEND_THREADS;
+    if (blocks > 0x7FFFFFFF) return cudaErrorInvalidConfiguration;
+    const dim3 grid(static_cast<unsigned>(blocks)), block(paged::APPEND_THREADS);
+    cudaError_t e = a.x_f32 ? launch_ex(paged::append_kernel<true>, grid, block, 0, stream, false, pdl, s, a, per_row,
                                         status_word(workspace))
-                            : launch_ex(paged::append_kernel<false>, grid, dim3(128), 0, stream, false, pdl, s, a,
+                            : launch_ex(paged::append_kernel<false>, grid, block, 0, stream, false, pdl, s, a, per_row,
                                         status_word(workspace));
     count_launch();
     return e;

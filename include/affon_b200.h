@@ -392,7 +392,7 @@ typedef enum affon_b200_rope {
  * q_out[row] and keys and values (from v_offset) to the row's slot.  qkv is
  * f32 or bf16; q_heads may be 0 (q_out unused).  A position outside the tables
  * or a slot outside the pool skips the row and is reported like a bad length.
- * Two rows of one call must not share a slot. */
+ * Two rows of one call must not share a slot, and q_out must not overlap qkv. */
 typedef struct affon_b200_append_desc {
     uint32_t struct_size;
     int32_t x_dtype;     /* AFFON_B200_F32 or AFFON_B200_BF16 */
