@@ -31,6 +31,14 @@ AFB_DEVICE float exp2_approx(float x) {
     return y;
 }
 
+// s0 += the low bf16 of u, s1 += the high one (f32 sums of mixed operands).
+AFB_DEVICE void add_bf16x2(float &s0, float &s1, uint32_t u) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+        "add.f32.bf16 %0, l, %0;\n\tadd.f32.bf16 %1, h, %1;\n\t}"
+        : "+f"(s0), "+f"(s1)
+        : "r"(u));
+}
+
 // (x0, x1) as bf16 pairs hi = bf16(x) and lo = bf16(x - hi): hi + lo carries
 // ~16 significant bits of x.
 AFB_DEVICE void split_bf16x2(float x0, float x1, uint32_t &hi, uint32_t &lo) {

@@ -326,7 +326,7 @@ AFB_DEVICE void tmem_ld_32x32b_x32(uint32_t taddr, uint32_t (&r)[32]) {
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(taddr));
 }
-// 16 and 32 consecutive columns per thread into tensor memory.
+// 16 consecutive columns per thread into tensor memory.
 AFB_DEVICE void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
@@ -338,13 +338,13 @@ AFB_DEVICE void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
 AFB_DEVICE void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // Makes every later use of r depend on this point of the (volatile) asm
 // sequence: after tmem_wait_ld(), for registers of a pending load.
-AFB_DEVICE void tie_regs(uint32_t (&r)[32]) {
+template <int N>
+AFB_DEVICE void tie_regs(uint32_t (&r)[N]) {
 #pragma unroll
-    for (int i = 0; i < 32; i += 16)
+    for (int i = 0; i < N; i += 8)
         asm volatile(""
                      : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]),
-                       "+r"(r[i + 6]), "+r"(r[i + 7]), "+r"(r[i + 8]), "+r"(r[i + 9]), "+r"(r[i + 10]), "+r"(r[i + 11]),
-                       "+r"(r[i + 12]), "+r"(r[i + 13]), "+r"(r[i + 14]), "+r"(r[i + 15]));
+                       "+r"(r[i + 6]), "+r"(r[i + 7]));
 }
 AFB_DEVICE void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 // The same wait, with the 16 registers of a pending tmem_ld_32x32b_x16 as

@@ -59,6 +59,9 @@ constexpr int PIECES = 4;           // pieces queued ahead
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float RAISE = 8.0f;       // log2: how far scores may pass the running maximum before it is raised
 
+// Named barriers: all softmax threads; a warpgroup's.
+constexpr int BAR_ALL = 1, BAR_GROUP = 2;
+
 template <int HD>
 struct Cfg {
     static constexpr int HALVES = HD / 64;
@@ -180,11 +183,6 @@ template <int N>
 __device__ __forceinline__ void tmem_ld_row(uint32_t taddr, uint32_t (&r)[N]) {
     if constexpr (N == 32) tmem_ld_32x32b_x32(taddr, r);
     else tmem_ld_32x32b_x16(taddr, r);
-}
-template <int N>
-__device__ __forceinline__ void tie_row(uint32_t (&r)[N]) {
-    if constexpr (N == 32) tie_regs(r);
-    else tmem_wait_ld(r);
 }
 
 // Rows row0 .. row0+rows-1 of a unit into a query buffer (K-major, 128-byte
@@ -654,7 +652,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
             if (both) {
                 mbar_wait(&q_empty[st], slots.parity(st) ^ 1, abort, p.status);
                 load_queries<HD>(p, d, st * TILE, min(TILE, d.rows - st * TILE), 0, qbuf + st * C::TILE_BYTES, r, 128);
-                named_bar_sync(2 + st, 128);
+                named_bar_sync(BAR_GROUP + st, 128);
                 if (r == 0) mbar_arrive(&q_full[st]);
             }
             float m = -INFINITY, l = 0.0f;
@@ -665,6 +663,12 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                 mbar_wait(&s_full[st], s_phase, abort, p.status);
                 s_phase ^= 1;
                 tc_fence_after();
+                uint32_t v0[32], v1[32];  // runs of 32 positions, the next one on its way while one is worked on
+                auto arrive = [&](uint32_t (&v)[32]) {
+                    tmem_wait_ld();
+                    tie_regs(v);
+                };
+                const bool single = k1 - k0 == 1;
                 if (warp_on) {
                     const int pos = (d.t0 + t) * TILE;
                     if (pos + 32 * k1 > d.ctx) {  // drafted positions, or the end: hidden scores become -inf
@@ -681,13 +685,6 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                         }
                         tmem_wait_st();
                     }
-                    // Runs of 32 positions, the next one on its way while one
-                    // is worked on.
-                    uint32_t v0[32], v1[32];
-                    auto arrive = [&](uint32_t (&v)[32]) {
-                        tmem_wait_ld();
-                        tie_regs(v);
-                    };
                     float top = -INFINITY;
                     auto raise_top = [&](const uint32_t (&v)[32]) {
                         float a[4];
@@ -697,7 +694,6 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                         for (int e = 4; e < 32; ++e) a[e & 3] = fmaxf(a[e & 3], __uint_as_float(v[e]));
                         top = fmaxf(top, fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])));
                     };
-                    const bool single = k1 - k0 == 1;
                     if (single) tmem_ld_32x32b_x32(ts + 32 * k0, v1);
                     else tmem_ld_32x32b_x32(ts + 32 * (k1 - 1), v0);
 #pragma unroll 1
@@ -737,8 +733,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                             const float a = exp2_approx(fmaf(__uint_as_float(x[2 * e]), sc, -off));
                             const float b = exp2_approx(fmaf(__uint_as_float(x[2 * e + 1]), sc, -off));
                             u[e] = pack_bf16x2(a, b);
-                            sum[0] += __uint_as_float(u[e] << 16);
-                            sum[1] += __uint_as_float(u[e] & 0xFFFF0000u);
+                            add_bf16x2(sum[0], sum[1], u[e]);
                         }
                         tmem_st_32x32b_x16(ts + 16 * run, u);  // over scores that have been read
                     };
@@ -779,7 +774,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
             if (!both) {  // join the streams' and copies' maxima and sums
                 float2 *ex = reinterpret_cast<float2 *>(scratch);
                 ex[st * TILE + r] = make_float2(m2, l);
-                named_bar_sync(1, SOFTMAX_THREADS);
+                named_bar_sync(BAR_ALL, SOFTMAX_THREADS);
                 const int states = 2 << copies, step = TILE >> copies;  // state i: stream i & 1, copy i >> 1
                 float2 e[8];
 #pragma unroll
@@ -795,7 +790,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                     lsum += e[i].y * wt;
                     if (i >> 1 == copy) (i & 1 ? w1 : w0) = wt;
                 }
-                named_bar_sync(1, SOFTMAX_THREADS);
+                named_bar_sync(BAR_ALL, SOFTMAX_THREADS);
             }
             const bool whole = d.t0 == 0 && d.t1 == d.nt;
             if (whole) {
@@ -823,8 +818,8 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                     tmem_ld_row<W>(to + (both ? st * HD : 0) + c, a);
                     if (pair) tmem_ld_row<W>(to + HD + c, b);
                     tmem_wait_ld();
-                    tie_row<W>(a);
-                    tie_row<W>(b);
+                    tie_regs(a);
+                    tie_regs(b);
 #pragma unroll
                     for (int e = 0; e < W; e += 4) {
                         float o[4];
@@ -836,7 +831,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                         if (mine) *cell(r, e / 4) = make_float4(o[0], o[1], o[2], o[3]);
                     }
                 }
-                named_bar_sync(2 + st, 128);
+                named_bar_sync(BAR_GROUP + st, 128);
 #pragma unroll 1
                 for (int i = r; i < rows * CH; i += 128) {
                     const int row = i / CH, k = i % CH;  // 8 dims of a row
@@ -856,7 +851,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                         dst[1] = make_float4(o[4], o[5], o[6], o[7]);
                     }
                 }
-                named_bar_sync(2 + st, 128);
+                named_bar_sync(BAR_GROUP + st, 128);
             }
             if (__any_sync(0xffffffffu, odd[lane & 7] != 0u) && mine && copy == 0) {
                 // Copies, so that what the call takes by address stays in registers elsewhere.
@@ -878,7 +873,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
             if (!whole) {
                 (d.t0 == 0 ? shares_start : shares_end) = true;
                 if (tid == 0) shared_units[d.t0 == 0] = d;
-                named_bar_sync(1, SOFTMAX_THREADS);
+                named_bar_sync(BAR_ALL, SOFTMAX_THREADS);
                 if (tid == 0) {  // the barrier's order and this fence publish all threads' stores
                     asm volatile("fence.acq_rel.gpu;" ::: "memory");
                     atomicAdd(&p.arrived[division->owner(d.start)], 1u);
@@ -957,11 +952,11 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                 }
                 if (parts > 1) {  // join the parts, in order, in the row's first
                     float *my = ex + tid;  // value e of a thread at ex[e * threads + thread]
-                    named_bar_sync(1, SOFTMAX_THREADS);
+                    named_bar_sync(BAR_ALL, SOFTMAX_THREADS);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) my[e * SOFTMAX_THREADS] = o[e];
                     my[8 * SOFTMAX_THREADS] = top, my[9 * SOFTMAX_THREADS] = lsum;
-                    named_bar_sync(1, SOFTMAX_THREADS);
+                    named_bar_sync(BAR_ALL, SOFTMAX_THREADS);
                     if (part == 0) {
 #pragma unroll 1
                         for (int i = 1; i < parts; ++i) top = fmaxf(top, my[8 * SOFTMAX_THREADS + i * CHUNKS]);
@@ -990,7 +985,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                 atomicExch(&p.arrived[owner0], 0u);
                 atomicExch(&p.done[owner0], 0u);
             }
-            named_bar_sync(1, SOFTMAX_THREADS);  // the next unit uses `ex` again
+            named_bar_sync(BAR_ALL, SOFTMAX_THREADS);  // the next unit uses `ex` again
         }
     }
     tc_fence_before();
