@@ -38,8 +38,8 @@ int check_desc(const affon_b200_paged_desc *d, afb::PagedShape *s) {
     const int64_t lim = int64_t(1) << 31;
     if (d->pages < 1 || d->pages > (lim - 1) / d->page_size)
         return fail(AFFON_B200_INVALID_SHAPE, "paged: pages must be positive, pages * page_size below 2^31");
-    if (d->ld_table < 1 || d->ld_table > (lim - 1) / d->page_size)
-        return fail(AFFON_B200_INVALID_SHAPE, "paged: ld_table must be positive, ld_table * page_size below 2^31");
+    if (d->ld_table < 1 || d->ld_table > (lim / 2 - 1) / d->page_size)
+        return fail(AFFON_B200_INVALID_SHAPE, "paged: ld_table must be positive, ld_table * page_size below 2^30");
     // A stride of a one-element axis is never used.
     *s = afb::PagedShape{d->seqs,  d->rows,        d->max_nodes,   d->kv_heads,     d->head_dim, shift, d->mask_words,
                          d->pages, d->page_stride, d->head_stride, d->token_stride, d->ld_table};

@@ -415,9 +415,13 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
             if (pos < end) {
                 while (at >= tiles) {
                     at = 0;
-                    q = seq_tiles(p, ++seq);
+                    if (++seq >= p.s.seqs) break;  // lengths that changed under the kernel
+                    q = seq_tiles(p, seq);
                     tiles = static_cast<int>(q.tiles(p.s.kv_heads));
                 }
+                if (seq >= p.s.seqs) pos = end;
+            }
+            if (pos < end) {
                 const int unit = at / q.nt;
                 d.seq = seq;
                 d.first = q.sp.first;

@@ -583,7 +583,7 @@ class PagedDecoder(QuantizedDecoder):
         dev = self.device
         i32 = lambda *shape: torch.zeros(shape, dtype=torch.int32, device=dev)
         per = -(-capacity // page_size)
-        self.page_table, self.ctx_lens, self.cu_nodes = i32(seqs, per), i32(seqs), i32(seqs + 1)
+        self.page_table, self.ctx_lens, self.cu_nodes = i32(seqs, per) - 1, i32(seqs), i32(seqs + 1)  # -1: no page
         self.parents, self.predicted = i32(rows), i32(rows)
         words = -(-self.max_nodes // 32)
         self.plan = TreePlan(i32(rows), i32(rows), i32(rows, words))
@@ -629,6 +629,7 @@ class PagedDecoder(QuantizedDecoder):
         """Return the sequence's pages; it holds nothing afterwards."""
         self._free += reversed(self._pages_of[seq])
         self._pages_of[seq] = []
+        self.page_table[seq] = -1
         self.ctx_lens[seq] = 0
 
     def set_step(self, nodes, parents=None, tokens=None):

@@ -363,7 +363,7 @@ typedef struct affon_b200_paged_desc {
     int32_t mask_words;  /* 32-bit words per row of the mask: ceil(max_nodes/32) at least, at most 8 */
     int64_t pages;       /* pages*page_size < 2^31 */
     int64_t page_stride, head_stride, token_stride; /* elements; multiples of 8, token_stride >= head_dim */
-    int64_t ld_table;    /* pages per row of page_table; ld_table*page_size < 2^31 */
+    int64_t ld_table;    /* pages per row of page_table; ld_table*page_size < 2^30 */
 } affon_b200_paged_desc;
 
 /* The descriptor's own rules (no GPU call). */
@@ -413,8 +413,10 @@ int affon_b200_paged_append(affon_b200_ctx *ctx, const affon_b200_paged_desc *de
  * nodes up to its own), and writes softmax(scale * q.k) v as bf16.  q and out
  * are bf16 [rows][q_heads*head_dim].  A row that sees nothing gets zeros;
  * padding rows are left as they were.  What a mask hides does not reach the
- * result, infinities and NaN included.  out must not overlap q or the caches.
- * The launch uses the context's workspace. */
+ * result, infinities and NaN included; what is visible and not finite makes
+ * the results that it reaches not finite (an infinite value may become NaN).
+ * out must not overlap q or the caches.  The launch uses the context's
+ * workspace; the lengths must not change while it runs. */
 typedef struct affon_b200_tree_attn_desc {
     uint32_t struct_size;
     int32_t q_heads;        /* a multiple of kv_heads */

@@ -41,7 +41,7 @@ def test_descriptor_accepts(kw):
     (dict(kv_heads=0), _lib.INVALID_SHAPE), (dict(head_dim=96), _lib.UNSUPPORTED),
     (dict(page_size=24), _lib.UNSUPPORTED), (dict(page_size=512), _lib.UNSUPPORTED), (dict(page_size=0), _lib.UNSUPPORTED),
     (dict(pages=0), _lib.INVALID_SHAPE), (dict(pages=1 << 27), _lib.INVALID_SHAPE),
-    (dict(ld_table=0), _lib.INVALID_SHAPE), (dict(ld_table=1 << 27), _lib.INVALID_SHAPE),
+    (dict(ld_table=0), _lib.INVALID_SHAPE), (dict(ld_table=1 << 26), _lib.INVALID_SHAPE),
     (dict(token_stride=64), _lib.INVALID_SHAPE), (dict(token_stride=132), _lib.INVALID_SHAPE),
     (dict(head_stride=0), _lib.INVALID_SHAPE), (dict(page_stride=-4096), _lib.INVALID_SHAPE),
     (dict(page_stride=1 << 39), _lib.INVALID_SHAPE)])

@@ -189,6 +189,18 @@ def test_pages_are_shared_out_and_overruns_reported():
         d.prefill([[], list(range(48))])
         d.synchronize()
         assert d.ctx_lens.tolist() == [0, 48]
+        # pages that a sequence gave back are not its any more, whatever its length says
+        d.release(1)
+        d.reserve(1, 10)
+        d.reserve(0, 10)
+        k0 = d.k_cache.clone()
+        d.ctx_lens[1] = 20
+        d.set_step([0, 1], tokens=[1])
+        d.step_eager()
+        with pytest.raises(AffonError):
+            d.synchronize()
+        assert torch.equal(d.k_cache, k0)
+        d.reset()
         k0 = d.k_cache.clone()
         d.ctx_lens[1] = 62                       # three more nodes pass the page table's end
         d.set_step([0, 3], tokens=[1, 2, 3])

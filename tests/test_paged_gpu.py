@@ -217,6 +217,30 @@ def test_attention_matches(sess, ctx, nodes, page, heads, group, hd):
     assert_close(st, *run_attention(sess, st, heads, group, hd, seed=hd + page))
 
 
+@pytest.mark.parametrize("ctx,nodes,page,heads,group,hd", [
+    ([20000], [1], 64, 1, 8, 128),               # one unit in a piece per SM
+    ([19000], [3], 16, 1, 20, 64),
+    ([5900, 4100], [200, 228], 128, 8, 8, 64),   # many pieces a CTA, units of 256, 64 and 32 rows in turn
+    ([900, 3, 2000], [70, 33, 129], 32, 3, 2, 128),
+    ([60, 200], [2, 3], 16, 1, 300, 128),        # more heads per KV head than a unit has rows
+    ([(i * 37) % 400 for i in range(300)], [1 + i % 5 if i % 7 else 0 for i in range(300)], 16, 2, 3, 64)])
+def test_attention_divides_any_work(sess, ctx, nodes, page, heads, group, hd):
+    st = ref.Step(ctx, nodes, page, seed=sum(nodes), pad=1)
+    assert_close(st, *run_attention(sess, st, heads, group, hd, seed=hd + len(ctx)))
+
+
+def test_visible_nan_keys_make_the_row_nan(sess):
+    st = ref.Step([150], [4], 16, parents=[np.array([-1, 0, 0, 2], dtype=np.int32)])
+    k, v = (t.cpu() for t in pools(st, 1, 64, 1))
+    pg, off = st.place(0, 152)                   # node 2, seen by nodes 2 and 3
+    k[0, pg, 0, off, 5] = math.nan
+    q = torch.randn((4, 64), generator=torch.Generator().manual_seed(3)).to(torch.bfloat16)
+    b = batch(sess, st, dev(k), dev(v))
+    got = paged.tree_attention(b, paged.TreePlan(None, None, dev(st.plan()[2])), dev(q), 1).cpu()
+    sess.synchronize()
+    assert torch.isfinite(got[:2]).all() and torch.isnan(got[2:]).all()
+
+
 @pytest.mark.parametrize("kw", [dict(nhd=True), dict(scale=0.3), dict(scale=-0.05), dict(sharp=30.0), dict(sharp=0.0), dict(pair=True)])
 def test_attention_variants(sess, kw):
     st = ref.Step([70, 400, 9], [9, 20, 1], 16, seed=8)
@@ -382,6 +406,45 @@ def test_attention_repeats_bit_for_bit_on_streams_and_in_graphs(sess):
     want = paged.tree_attention(b, plan, q, 16)
     sess.synchronize()
     assert torch.equal(out, want) and not torch.equal(out, first)
+
+
+def test_sessions_on_two_streams_do_not_disturb_each_other():
+    """A Session per stream: both attend at once, neither sees the other's workspace."""
+    st = ref.Step([2500, 900, 40], [5, 9, 1], 16, seed=6)
+    k, v = pools(st, 4, 128, 0)
+    q = torch.randn((st.rows, 16 * 128), device=DEV).to(torch.bfloat16)
+    plan = paged.TreePlan(None, None, dev(st.plan()[2]))
+    with Session("cuda:0") as one, Session("cuda:0") as two:
+        want = paged.tree_attention(batch(one, st, k, v), plan, q, 16)
+        one.synchronize()
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        outs = []
+        for s, stream in zip((one, two), streams):
+            stream.wait_stream(torch.cuda.current_stream())
+            b = batch(s, st, k, v)
+            with torch.cuda.stream(stream):
+                outs.append([paged.tree_attention(b, plan, q, 16) for _ in range(20)])
+        for s in (one, two):
+            s.synchronize()
+        assert all(torch.equal(o, want) for group in outs for o in group)
+
+
+def test_disposed_session_and_zero_scale_are_refused(sess):
+    st = ref.Step([5], [1], 16)
+    k, v = pools(st, 1, 64, 0)
+    b = batch(sess, st, k, v)
+    q = torch.zeros((1, 64), dtype=torch.bfloat16, device=DEV)
+    for scale in (0.0, math.inf, math.nan):
+        with pytest.raises(AffonError) as err:
+            paged.tree_attention(b, None, q, 1, scale=scale)
+        assert err.value.code == "invalid_arg"
+    gone = Session("cuda:0")
+    b = batch(gone, st, k, v)
+    gone.dispose()
+    with pytest.raises(AffonError):
+        paged.tree_attention(b, None, q, 1)
+    with pytest.raises(AffonError):
+        gone.synchronize()
 
 
 # ----------------------------------------------------------------- accept
