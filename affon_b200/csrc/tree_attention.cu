@@ -25,19 +25,31 @@
 // sum: units of more than 128 rows give each its own 128 rows and both take
 // every tile; smaller units give both the same rows and they take alternate
 // tiles.  While one stream is in its softmax the tensor cores work for the
-// other.  Units of at most 64 (16) rows fill the 128 rows of the MMA with 2
+// other.  Units of at most 64 (32) rows fill the 128 rows of the MMA with 2
 // (4) copies, and each copy's warps take half (a quarter) of a tile's
 // positions: the softmax of few rows then runs on all warps.  The streams'
 // and copies' results are joined when the piece ends.
 //
 // A row's maximum is only raised (and O rescaled) when it grows by more than
-// 2^8, so O is rarely touched.  The loops over a tile's columns and a row's
-// dims stay rolled: code that runs once per launch is bound by its fetching.
+// 2^8, so O is rarely touched.  Hidden scores are cleared in tensor memory
+// before the softmax of the few tiles that have any, which keeps the masks out
+// of the common path.
 //
 // Rounding: P is rounded to bf16 for the tensor cores (as V is bf16, it is the
 // smaller part of the result's own rounding); the sum l adds the rounded
 // values, so a row's weights still sum to one.  Scores, maxima, sums and O are
 // f32.
+//
+// Bounds.  Units of up to 128 rows are bound by HBM once a CTA has enough
+// tiles: 64 rows on 4 x 128K positions (2.06 GB) take 317 us, 6.5 TB/s, 0.99 of
+// the measured copy rate.  Units of 129 to 256 rows are bound by the
+// exponentials: a warp's 128 a row (8 cycles each) hardly overlap with its
+// other instructions, 2.9 us a tile where the products take 1.2 and the
+// tile's bytes 1.4.  (8 x 8K positions under 60 drafts, 256 rows: 113 us.
+// Two warps a row, turns between the streams, items of half a tile and all
+// scores in registers measured 114, 123, 126 and 119.)  Short contexts are
+// bound by latency: 4.5 us to the first scores, 2.5 to store a piece, 4 to
+// merge a unit (16 x 1000 positions, one node each: 27.6 us).
 #include <cuda_runtime.h>
 
 #include "common.cuh"

@@ -122,7 +122,7 @@ int affon_b200_ctx_destroy(affon_b200_ctx *ctx);
 int affon_b200_ctx_set_stream(affon_b200_ctx *ctx, void *cuda_stream);
 int affon_b200_ctx_device(const affon_b200_ctx *ctx);
 /* Overlap mode (default off): launch the decode kernels (qmv, its prologue,
- * decode attention, embed, finalize) with programmatic dependent launch, so
+ * decode attention, embed, finalize, the paged-cache kernels) with programmatic dependent launch, so
  * each may start while the kernel before it in the stream finishes and
  * prefetch its weights, scales and biases -- never its activations -- before
  * waiting for that kernel.  Enable it only when no kernel launched directly
