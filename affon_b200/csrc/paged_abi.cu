@@ -101,9 +101,9 @@ int affon_b200_paged_append(affon_b200_ctx *ctx, const affon_b200_paged_desc *de
     const int64_t per = d->x_dtype == AFFON_B200_F32 ? 4 : 8;  // elements of 16 bytes
     const int64_t begin[3] = {d->q_offset, d->k_offset, d->v_offset}, cols[3] = {q_cols, kv_cols, kv_cols};
     for (int i = d->q_heads ? 0 : 1; i < 3; ++i)
-        if (begin[i] < 0 || begin[i] % per || begin[i] + cols[i] > d->ld_qkv)
+        if (begin[i] < 0 || begin[i] % per || begin[i] + cols[i] > d->ld_qkv || begin[i] + cols[i] > 0x7FFFFFFF)
             return fail(AFFON_B200_INVALID_SHAPE, "paged_append: query, key and value columns must be 16-byte aligned "
-                                                  "and lie inside a row of qkv");
+                                                  "and lie inside a row of qkv, before its column 2^31");
     if (d->ld_qkv % per) return fail(AFFON_B200_INVALID_SHAPE, "paged_append: rows of qkv must be 16-byte aligned");
     if (d->q_heads && (d->ld_q < q_cols || d->ld_q % 8))
         return fail(AFFON_B200_INVALID_SHAPE, "paged_append: ld_q must be a multiple of 8 and hold q_heads heads");
@@ -149,8 +149,8 @@ int affon_b200_tree_attention(affon_b200_ctx *ctx, const affon_b200_paged_desc *
         return fail(AFFON_B200_INVALID_ARG, "tree_attention: null context or bad descriptor");
     if (d->q_heads < 1 || d->q_heads > 65536 || d->q_heads % s.kv_heads)
         return fail(AFFON_B200_INVALID_SHAPE, "tree_attention: q_heads must be a multiple of kv_heads, at most 65536");
-    if (!(d->scale > -3.0e38f && d->scale < 3.0e38f) || d->scale == 0.0f)
-        return fail(AFFON_B200_INVALID_ARG, "tree_attention: scale must be finite and not zero");
+    if (!(d->scale > -2.0e38f && d->scale < 2.0e38f) || d->scale == 0.0f)  // scale * log2(e) is finite, too
+        return fail(AFFON_B200_INVALID_ARG, "tree_attention: scale must be below 2e38 in magnitude and not zero");
     const int64_t cols = int64_t(d->q_heads) * s.head_dim;
     if (d->ld_q < cols || d->ld_out < cols || d->ld_q % 8 || d->ld_out % 8)
         return fail(AFFON_B200_INVALID_SHAPE, "tree_attention: ld_q and ld_out must be multiples of 8 and hold q_heads "

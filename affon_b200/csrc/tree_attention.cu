@@ -319,6 +319,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
     uint32_t *odd = reinterpret_cast<uint32_t *>(division + 1);  // drafted nodes whose values are not all finite
     uint32_t *tmem_addr = odd + kMaxTreeNodes / 32;
     volatile int *abort = reinterpret_cast<volatile int *>(tmem_addr + 1);
+    volatile uint32_t *closed = tmem_addr + 2;  // how many pieces were queued, known at the end
 
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // warp-uniform for the compiler, too
@@ -340,6 +341,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
         mbar_init(unit_done, 2);
         mbar_init(o_free, SOFTMAX_WARPS);
         *abort = 0;
+        *closed = 0xFFFFFFFFu;
         fence_mbar_init();
     }
     if (warp == MMA) {
@@ -358,11 +360,19 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
     const uint32_t tmem = static_cast<uint32_t>(uniform(static_cast<int>(*tmem_addr)));
 
     // The next piece of the queue (all threads of a warp); rows 0 at its end
-    // or after an abort.
+    // or after an abort.  The softmax warps meet at barriers, so all of them
+    // take every piece that was queued, abort or not: they leave only once the
+    // scheduler, whose own waits are bounded, has closed the queue.
     uint32_t taken = 0;
     auto next_piece = [&](Piece &d) {
         const uint32_t i = taken++;
-        const bool ok = warp_wait(&d_full[i % PIECES], (i / PIECES) & 1, abort, p.status);
+        bool ok;
+        if (warp < SOFTMAX_WARPS) {
+            while (!(ok = mbar_try_wait(&d_full[i % PIECES], (i / PIECES) & 1)) && i < *closed) {}
+            ok = __all_sync(0xffffffffu, ok);
+        } else {
+            ok = warp_wait(&d_full[i % PIECES], (i / PIECES) & 1, abort, p.status);
+        }
         d = queue[i % PIECES];
         d.rows = uniform(ok ? d.rows : 0);
         __syncwarp();
@@ -419,6 +429,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                 before += __shfl_sync(0xffffffffu, upto, 31);
             }
         }
+        uint32_t queued = 0;
         SeqTiles q{};
         int tiles = 0;
         if (pos < end) q = seq_tiles(p, seq), tiles = static_cast<int>(q.tiles(p.s.kv_heads));
@@ -456,8 +467,10 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                 mbar_arrive(&d_full[i % PIECES]);
             }
             __syncwarp();
+            queued = i + 1;
             if (d.rows == 0) break;
         }
+        if (lane == 0) *closed = queued;
     } else if (warp == QUERIES) {  // ---------------------------------------------- query rows
         QuerySlots slots;
         Piece d;

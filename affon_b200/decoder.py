@@ -576,6 +576,8 @@ class PagedDecoder(QuantizedDecoder):
                  workspace_bytes=None, overlap=True):
         if not 1 <= seqs <= rows:
             raise ValueError("a step needs a row for each of its 1 or more sequences")
+        if page_size not in (16, 32, 64, 128, 256):
+            raise ValueError("page_size must be 16, 32, 64, 128 or 256")
         self.seqs, self.page_size, self.pages = seqs, page_size, pages
         self.max_nodes = min(rows, max_nodes or rows)
         super().__init__(cfg, rows, capacity, device, seed=seed, max_steps=1, workspace_bytes=workspace_bytes,
@@ -643,6 +645,8 @@ class PagedDecoder(QuantizedDecoder):
             cu.append(cu[-1] + n)
         if parents is None:
             parents = [i - 1 for n in nodes for i in range(n)]
+        if len(parents) != cu[-1] or tokens is not None and len(tokens) != cu[-1]:
+            raise ValueError(f"parents and tokens must have an entry for each of the {cu[-1]} nodes")
         host = lambda v: torch.as_tensor(v, dtype=torch.int32)
         self.cu_nodes.copy_(host(cu))
         self.parents[:cu[-1]] = host(parents).to(self.device)

@@ -18,9 +18,9 @@ replayed on changed contents.  What the kernels find wrong with them is
 reported by `Session.synchronize()`.
 
 Calls run on the Session's device and on torch's current stream of it.
-`tree_attention` uses the Session's workspace: attention calls of one Session
-(and graphs captured from them) must not run at the same time on two streams;
-make a Session per stream for that.  The reference has no counterpart: its
+`tree_attention` and `tree_accept` use the Session's workspace: such calls of one
+Session (and graphs captured from them) must not run at the same time on two
+streams; make a Session per stream for that.  The reference has no counterpart: its
 models use a fixed-capacity cache.
 """
 import ctypes

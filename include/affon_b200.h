@@ -122,11 +122,14 @@ int affon_b200_ctx_destroy(affon_b200_ctx *ctx);
 int affon_b200_ctx_set_stream(affon_b200_ctx *ctx, void *cuda_stream);
 int affon_b200_ctx_device(const affon_b200_ctx *ctx);
 /* Overlap mode (default off): launch the decode kernels (qmv, its prologue,
- * decode attention, embed, finalize, the paged-cache kernels) with programmatic dependent launch, so
- * each may start while the kernel before it in the stream finishes and
- * prefetch its weights, scales and biases -- never its activations -- before
- * waiting for that kernel.  Enable it only when no kernel launched directly
- * before one of these writes its weights, scales or biases. */
+ * decode attention, embed, finalize, the paged-cache kernels) with
+ * programmatic dependent launch, so each may start while the kernel before it
+ * in the stream finishes and prefetch its weights, scales and biases -- never
+ * its activations -- before waiting for that kernel.  Enable it only when no
+ * kernel launched directly before one of these writes its weights, scales or
+ * biases, and on one context of a GPU at a time: a kernel whose CTAs wait for
+ * one another is then not launched cooperatively, so two of them could each
+ * hold a part of the SMs (both would give up: AFFON_B200_TIMEOUT). */
 int affon_b200_ctx_set_overlap(affon_b200_ctx *ctx, int enable);
 
 /* Test hook of the decode qmv's split-K combine, process-wide: the limit of
@@ -414,13 +417,15 @@ int affon_b200_paged_append(affon_b200_ctx *ctx, const affon_b200_paged_desc *de
  * are bf16 [rows][q_heads*head_dim].  A row that sees nothing gets zeros;
  * padding rows are left as they were.  What a mask hides does not reach the
  * result, infinities and NaN included; what is visible and not finite makes
- * the results that it reaches not finite (an infinite value may become NaN).
- * out must not overlap q or the caches.  The launch uses the context's
- * workspace; the lengths must not change while it runs. */
+ * the results that it reaches not finite (an infinite value may become NaN;
+ * a position whose score is minus infinity has no weight).  A step has at most
+ * 2^30 tiles of 128 positions x 256 rows of a KV head.  out must not overlap q
+ * or the caches.  The launch uses the context's workspace; the lengths must
+ * not change while it runs. */
 typedef struct affon_b200_tree_attn_desc {
     uint32_t struct_size;
     int32_t q_heads;        /* a multiple of kv_heads */
-    float scale;            /* finite, not zero */
+    float scale;            /* below 2e38 in magnitude, not zero */
     int32_t out_pair_order; /* write the output in 4-bit qmv pair order */
     int64_t ld_q, ld_out;
 } affon_b200_tree_attn_desc;
@@ -441,7 +446,8 @@ int affon_b200_tree_attention(affon_b200_ctx *ctx, const affon_b200_paged_desc *
  * together, from position ctx_lens[s]+path[i] to ctx_lens[s]+i, in `layers`
  * caches that lie layer_stride elements apart.  A sequence without nodes gets
  * count 0, next token -1 and keeps its length.  lens_out may be ctx_lens.
- * parents == NULL: chains.  layers 0 moves nothing (the caches may be NULL). */
+ * parents == NULL: chains.  layers 0 moves nothing (the caches may be NULL).
+ * The launch uses the context's workspace, as tree_attention does. */
 int affon_b200_tree_accept(affon_b200_ctx *ctx, const affon_b200_paged_desc *desc, int layers, int64_t layer_stride,
                            const int *cu_nodes, const int *parents, const int *tokens, const int *predicted,
                            const int *page_table, const int *ctx_lens, void *k_cache, void *v_cache, int *counts,

@@ -184,6 +184,10 @@ def test_pages_are_shared_out_and_overruns_reported():
             d.reserve(1, 65)
         with pytest.raises(ValueError):
             d.set_step([3, 2])
+        with pytest.raises(ValueError):
+            d.set_step([2, 2], parents=[-1])
+        with pytest.raises(ValueError):
+            d.set_step([2, 2], tokens=[1, 2, 3])
         d.release(0)
         d.reserve(1, 48)
         d.prefill([[], list(range(48))])

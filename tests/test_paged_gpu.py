@@ -447,6 +447,35 @@ def test_disposed_session_and_zero_scale_are_refused(sess):
         gone.synchronize()
 
 
+def test_scales_whose_log2_form_overflows_are_refused(sess):
+    st = ref.Step([5], [1], 16)
+    k, v = pools(st, 1, 64, 0)
+    b = batch(sess, st, k, v)
+    q = torch.zeros((1, 64), dtype=torch.bfloat16, device=DEV)
+    for scale in (3.0e38, -3.0e38):
+        with pytest.raises(AffonError) as err:
+            paged.tree_attention(b, None, q, 1, scale=scale)
+        assert err.value.code == "invalid_arg"
+    v.normal_()
+    want = v[0, int(st.table[0, 0]), 0, :6].double().mean(0)     # equal scores: the mean of the values
+    for scale in (1.9e38, -1.9e38):
+        out = paged.tree_attention(b, None, q, 1, scale=scale)
+        sess.synchronize()
+        # one rounding of the result (2^-8 of it, half a step with room) and an f32 sum
+        assert ((out[0].double() - want).abs() <= 2 ** -8 * want.abs() + 1e-5).all()
+
+
+def test_append_refuses_columns_past_31_bits(sess):
+    import ctypes
+    from affon_b200 import _lib
+    st = ref.Step([5], [1], 16)
+    k, v = pools(st, 1, 64, 0)
+    b = batch(sess, st, k, v)
+    d = _lib.AppendDesc(ctypes.sizeof(_lib.AppendDesc), _lib.BF16, 0, 1, 0, 64, 2 ** 31 - 64, 1, 2 ** 33, 64)
+    status = _lib.lib().affon_b200_paged_append(sess._ctx, ctypes.byref(b.desc), ctypes.byref(d), *[None] * 8)
+    assert status == _lib.INVALID_SHAPE
+
+
 # ----------------------------------------------------------------- accept
 def accept_case(st, rng, follow=0.8):
     """Tokens and predictions that accept paths of different lengths (with repeated sibling tokens)."""
