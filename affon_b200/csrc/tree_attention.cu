@@ -15,6 +15,11 @@
 // and the start of another; whole units are finished in place, pieces go to
 // the workspace and the CTAs that share a unit merge it together at the end,
 // each a share of its rows, in piece order (results do not depend on timing).
+// A second piece costs a CTA about 2.5 us and a merge 4, as much as several
+// tiles, so where there are no more units than CTAs the scheduler weighs equal
+// shares against one piece for each CTA, and against whole units without any
+// merge (5 trees of 4 to 16 tiles, 8 KV heads: 28 -> 20 us with pieces, 34
+// whole; 16 sequences of 6 to 11 tiles: 28 -> 22 whole).
 //
 // Roles.  A scheduler warp reads the lengths and queues the CTA's pieces; a
 // query warp copies their rows ahead of time; a producer warp brings K and V
@@ -49,7 +54,7 @@
 // Two warps a row, turns between the streams, items of half a tile and all
 // scores in registers measured 114, 123, 126 and 119.)  Short contexts are
 // bound by latency: 4.5 us to the first scores, 2.5 to store a piece, 4 to
-// merge a unit (16 x 1000 positions, one node each: 27.6 us).
+// merge a unit (16 x 1000 positions, one node each: 21.8 us).
 #include <cuda_runtime.h>
 
 #include "common.cuh"
@@ -68,6 +73,9 @@ constexpr int THREADS = 32 * 12;
 constexpr int SOFTMAX_THREADS = 32 * SOFTMAX_WARPS;
 constexpr int HALF_BYTES = TILE * 128;  // 64 dims of a tile
 constexpr int PIECES = 4;           // pieces queued ahead
+// What the scheduler weighs, in measured 0.1 us: a tile of units of up to 128
+// (256) rows, the end of a piece, the merge of a unit.
+constexpr int TILE_COST = 13, TILE2_COST = 29, PIECE_COST = 25, MERGE_COST = 40;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float RAISE = 8.0f;       // log2: how far scores may pass the running maximum before it is raised
 
@@ -121,7 +129,7 @@ struct Shares {
 // A piece of a unit: tiles [t0, t1) of nt.  rows 0 ends the queue.
 struct Piece {
     int seq, first, n, ctx, kv, row0, rows, t0, t1, nt;
-    int start;  // the unit's first tile in the order of all tiles
+    int owner0, owners;  // the CTAs that share the unit
     __device__ __forceinline__ bool both() const { return rows > TILE; }  // two row tiles, every position tile for both
     // log2 of the copies of the rows in the 128 rows of the MMA.
     __device__ __forceinline__ int copies() const { return rows <= 32 ? 2 : rows <= 64 ? 1 : 0; }
@@ -315,8 +323,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
     uint64_t *o_free = unit_done + 1;        // its O has been read
     Piece *queue = reinterpret_cast<Piece *>(o_free + 1);
     Piece *shared_units = queue + PIECES;    // [2] pieces of shared units: the end of one, the start of another
-    Shares *division = reinterpret_cast<Shares *>(shared_units + 2);
-    uint32_t *odd = reinterpret_cast<uint32_t *>(division + 1);  // drafted nodes whose values are not all finite
+    uint32_t *odd = reinterpret_cast<uint32_t *>(shared_units + 2);  // drafted nodes whose values are not all finite
     uint32_t *tmem_addr = odd + kMaxTreeNodes / 32;
     volatile int *abort = reinterpret_cast<volatile int *>(tmem_addr + 1);
     volatile uint32_t *closed = tmem_addr + 2;  // how many pieces were queued, known at the end
@@ -382,11 +389,12 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
 
     if (warp == SCHEDULER) {  // ------------------------------------------------- the CTA's pieces
         unsigned total = 0, mine = 0, high = 0;  // high: the total / 1024, should it not fit
+        SeqTiles q{};
         for (int base = 0; base < p.s.seqs; base += 32) {
             mine = 0;
             unsigned part = 0;
             if (base + lane < p.s.seqs) {
-                const SeqTiles q = seq_tiles(p, base + lane);
+                q = seq_tiles(p, base + lane);
                 const int64_t tiles = q.tiles(p.s.kv_heads);
                 mine = static_cast<unsigned>(tiles);
                 part = static_cast<unsigned>(min(tiles >> 10, int64_t(1) << 26));
@@ -403,8 +411,50 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
         sh.grid = min(static_cast<int>(total), static_cast<int>(gridDim.x));
         sh.per = sh.grid ? static_cast<int>(total) / sh.grid : 0;
         sh.extra = static_cast<int>(total) - sh.per * sh.grid;
-        int pos = 0, end = 0, seq = 0, at = 0;
-        if (static_cast<int>(blockIdx.x) < sh.grid) {
+        // With few units a piece each for every CTA may be better than equal
+        // numbers of tiles.  Weighed for up to 32 sequences, a lane each.
+        int pieces = 0;  // of the lane's sequence's units, 0: equal shares
+        if (p.s.seqs <= 32 && total) {
+            const int units = q.nt ? p.s.kv_heads * q.units : 0;
+            const int longest = __reduce_max_sync(0xffffffffu, q.nt);
+            if (__reduce_add_sync(0xffffffffu, units) <= gridDim.x) {
+                const int cost = __any_sync(0xffffffffu, q.n * p.group > TILE) ? TILE2_COST : TILE_COST;
+                const int even = sh.per + (sh.extra > 0);
+                int best = even * cost + PIECE_COST + MERGE_COST;
+#pragma unroll 1
+                for (int c = even; c < longest && c * cost + MERGE_COST < best; ++c) {
+                    const int n = q.nt ? (q.nt + c - 1) / c : 0;
+                    if (__reduce_add_sync(0xffffffffu, units * n) <= gridDim.x) {
+                        best = c * cost + MERGE_COST;
+                        pieces = n;
+                    }
+                }
+                if (longest * cost < best) pieces = q.nt ? 1 : 0;
+            }
+        }
+        const bool single = __any_sync(0xffffffffu, pieces > 0);
+        int pos = 0, end = 0, seq = 0, at = 0, owners = 0;
+        if (single) {
+            mine = pieces * p.s.kv_heads * q.units;
+            int upto = static_cast<int>(mine);
+#pragma unroll 1
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += v;
+            }
+            const unsigned past = __ballot_sync(0xffffffffu, upto > static_cast<int>(blockIdx.x));
+            if (past) {
+                seq = __ffs(past) - 1;
+                at = blockIdx.x - __shfl_sync(0xffffffffu, upto - static_cast<int>(mine), seq);
+                owners = __shfl_sync(0xffffffffu, pieces, seq);
+                end = 1;
+            }
+            q.sp.first = __shfl_sync(0xffffffffu, q.sp.first, seq);
+            q.sp.ctx = __shfl_sync(0xffffffffu, q.sp.ctx, seq);
+            q.n = __shfl_sync(0xffffffffu, q.n, seq);
+            q.units = __shfl_sync(0xffffffffu, q.units, seq);
+            q.nt = __shfl_sync(0xffffffffu, q.nt, seq);
+        } else if (static_cast<int>(blockIdx.x) < sh.grid) {
             pos = sh.begin(blockIdx.x);
             end = sh.begin(blockIdx.x + 1);
             int before = 0;
@@ -430,12 +480,11 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
             }
         }
         uint32_t queued = 0;
-        SeqTiles q{};
         int tiles = 0;
-        if (pos < end) q = seq_tiles(p, seq), tiles = static_cast<int>(q.tiles(p.s.kv_heads));
+        if (pos < end && !single) q = seq_tiles(p, seq), tiles = static_cast<int>(q.tiles(p.s.kv_heads));
         for (uint32_t i = 0;; ++i) {
             Piece d{};
-            if (pos < end) {
+            if (pos < end && !single) {
                 while (at >= tiles) {
                     at = 0;
                     if (++seq >= p.s.seqs) break;  // lengths that changed under the kernel
@@ -445,24 +494,32 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                 if (seq >= p.s.seqs) pos = end;
             }
             if (pos < end) {
-                const int unit = at / q.nt;
+                const int unit = at / (single ? owners : q.nt);
                 d.seq = seq;
                 d.first = q.sp.first;
                 d.n = q.n;
                 d.ctx = q.sp.ctx;
                 d.nt = q.nt;
-                d.t0 = at - unit * q.nt;
-                d.t1 = min(q.nt, d.t0 + end - pos);
+                if (single) {
+                    const int j = at - unit * owners;
+                    d.t0 = q.nt * j / owners;
+                    d.t1 = q.nt * (j + 1) / owners;
+                    d.owner0 = blockIdx.x - j;
+                    d.owners = owners;
+                } else {
+                    d.t0 = at - unit * q.nt;
+                    d.t1 = min(q.nt, d.t0 + end - pos);
+                    d.owner0 = sh.owner(pos - d.t0);
+                    d.owners = sh.owner(pos - d.t0 + q.nt - 1) - d.owner0 + 1;
+                }
                 d.kv = unit / q.units;
                 d.row0 = (unit - d.kv * q.units) * ROWS;
                 d.rows = min(ROWS, q.n * p.group - d.row0);
-                d.start = pos - d.t0;
-                pos += d.t1 - d.t0;
                 at += d.t1 - d.t0;
+                pos = single ? end : pos + d.t1 - d.t0;
             }
             if (!warp_wait(&d_empty[i % PIECES], ((i / PIECES) & 1) ^ 1, abort, p.status)) break;
             if (lane == 0) {
-                if (i == 0) *division = sh;
                 queue[i % PIECES] = d;
                 mbar_arrive(&d_full[i % PIECES]);
             }
@@ -905,7 +962,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                 named_bar_sync(BAR_ALL, SOFTMAX_THREADS);
                 if (tid == 0) {  // the barrier's order and this fence publish all threads' stores
                     asm volatile("fence.acq_rel.gpu;" ::: "memory");
-                    atomicAdd(&p.arrived[division->owner(d.start)], 1u);
+                    atomicAdd(&p.arrived[d.owner0], 1u);
                 }
             }
         }
@@ -915,7 +972,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
         for (int which = 0; which < 2; ++which) {
             if (!(which ? shares_start : shares_end)) continue;
             const Piece u = shared_units[which];
-            const int owner0 = division->owner(u.start), k = division->owner(u.start + u.nt - 1) - owner0 + 1;
+            const int owner0 = u.owner0, k = u.owners;
             const int me = blockIdx.x - owner0;
             const int r0 = u.rows * me / k, rows = u.rows * (me + 1) / k - r0;
             bool ok = true;

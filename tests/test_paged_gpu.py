@@ -229,6 +229,18 @@ def test_attention_divides_any_work(sess, ctx, nodes, page, heads, group, hd):
     assert_close(st, *run_attention(sess, st, heads, group, hd, seed=hd + len(ctx)))
 
 
+@pytest.mark.parametrize("ctx,nodes,page,heads,group,hd", [
+    ([1021, 2111, 1500, 1800, 1207], [3, 7, 5, 4, 6], 16, 8, 8, 128),   # a piece for each CTA
+    ([700 + 40 * i for i in range(16)], [1] * 16, 64, 8, 4, 128),       # whole units
+    ([900, 1200], [64, 50], 32, 8, 4, 128),                             # two row tiles
+    ([600, 0, 35, 2500], [9, 0, 129, 2], 64, 3, 2, 64),                 # sequences without nodes between
+    ([250 + i for i in range(32)], [1] * 32, 32, 4, 2, 64),             # 32 sequences are weighed,
+    ([250 + i for i in range(33)], [1] * 33, 32, 4, 2, 64)])            # 33 are not
+def test_attention_of_few_units(sess, ctx, nodes, page, heads, group, hd):
+    st = ref.Step(ctx, nodes, page, seed=sum(nodes) + 1, pad=2)
+    assert_close(st, *run_attention(sess, st, heads, group, hd, seed=hd + len(ctx)))
+
+
 def test_visible_nan_keys_make_the_row_nan(sess):
     st = ref.Step([150], [4], 16, parents=[np.array([-1, 0, 0, 2], dtype=np.int32)])
     k, v = (t.cpu() for t in pools(st, 1, 64, 1))
