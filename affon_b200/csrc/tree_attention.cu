@@ -35,10 +35,15 @@
 // positions: the softmax of few rows then runs on all warps.  The streams'
 // and copies' results are joined when the piece ends.
 //
-// A row's maximum is only raised (and O rescaled) when it grows by more than
-// 2^8, so O is rarely touched.  Hidden scores are cleared in tensor memory
-// before the softmax of the few tiles that have any, which keeps the masks out
-// of the common path.
+// A row's maximum is only raised when a score passes it by more than 2^8, and
+// then by a whole power of two: the sums, the tile's probabilities so far and
+// O are rescaled without another rounding, and rarely.  So a run of 32 scores
+// is read once, and little code does for all of it: short contexts wait for
+// instructions as much as for data (a pass for the maximum before the one for
+// the exponentials, with loads ahead, took 12.8 us instead of 11.7 for one
+// token, 20.2 instead of 18.0 for 5 small trees, 114 instead of 113 for wide
+// ones).  Hidden scores are cleared in tensor memory before the softmax of the
+// few tiles that have any, which keeps the masks out of the common path.
 //
 // Rounding: P is rounded to bf16 for the tensor cores (as V is bf16, it is the
 // smaller part of the result's own rounding); the sum l adds the rounded
@@ -46,7 +51,7 @@
 // f32.
 //
 // Bounds.  Units of up to 128 rows are bound by HBM once a CTA has enough
-// tiles: 64 rows on 4 x 128K positions (2.06 GB) take 317 us, 6.5 TB/s, 0.99 of
+// tiles: 64 rows on 4 x 128K positions (2.06 GB) take 315 us, 6.5 TB/s, 0.99 of
 // the measured copy rate.  Units of 129 to 256 rows are bound by the
 // exponentials: a warp's 128 a row (8 cycles each) hardly overlap with its
 // other instructions, 2.9 us a tile where the products take 1.2 and the
@@ -54,7 +59,7 @@
 // Two warps a row, turns between the streams, items of half a tile and all
 // scores in registers measured 114, 123, 126 and 119.)  Short contexts are
 // bound by latency: 4.5 us to the first scores, 2.5 to store a piece, 4 to
-// merge a unit (16 x 1000 positions, one node each: 21.8 us).
+// merge a unit (16 x 1000 positions, one node each: 20.4 us).
 #include <cuda_runtime.h>
 
 #include "common.cuh"
@@ -741,7 +746,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                 named_bar_sync(BAR_GROUP + st, 128);
                 if (r == 0) mbar_arrive(&q_full[st]);
             }
-            float m = -INFINITY, l = 0.0f;
+            float off = -INFINITY, l = 0.0f;  // the maximum that is weighed against, in log2 units, and the sum
             const int nt = d.t1 - d.t0, stride = both ? 1 : 2;
             const int k0 = copy << (2 - copies), k1 = (copy + 1) << (2 - copies);  // this copy's runs of 32 positions
 #pragma unroll 1
@@ -749,12 +754,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                 mbar_wait(&s_full[st], s_phase, abort, p.status);
                 s_phase ^= 1;
                 tc_fence_after();
-                uint32_t v0[32], v1[32];  // runs of 32 positions, the next one on its way while one is worked on
-                auto arrive = [&](uint32_t (&v)[32]) {
-                    tmem_wait_ld();
-                    tie_regs(v);
-                };
-                const bool single = k1 - k0 == 1;
+                uint32_t v[32];  // a run of 32 positions
                 if (warp_on) {
                     const int pos = (d.t0 + t) * TILE;
                     if (pos + 32 * k1 > d.ctx) {  // drafted positions, or the end: hidden scores become -inf
@@ -771,33 +771,40 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                         }
                         tmem_wait_st();
                     }
-                    float top = -INFINITY;
-                    auto raise_top = [&](const uint32_t (&v)[32]) {
+                    float sum[2] = {0.0f, 0.0f};  // of the tile: a long sum of sums loses less
+                    // Raises the maximum if a score of this run asks for it.
+                    auto look = [&](const uint32_t (&x)[32], int run) {
                         float a[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) a[e] = __uint_as_float(v[e]);
+                        for (int e = 0; e < 4; ++e) a[e] = __uint_as_float(x[e]);
 #pragma unroll
-                        for (int e = 4; e < 32; ++e) a[e & 3] = fmaxf(a[e & 3], __uint_as_float(v[e]));
-                        top = fmaxf(top, fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])));
-                    };
-                    if (single) tmem_ld_32x32b_x32(ts + 32 * k0, v1);
-                    else tmem_ld_32x32b_x32(ts + 32 * (k1 - 1), v0);
-#pragma unroll 1
-                    for (int k = k1 - 1; k >= k0; k -= 2) {  // downwards: run k0 ends up in v1
-                        if (!single) {
-                            arrive(v0);
-                            tmem_ld_32x32b_x32(ts + 32 * (k - 1), v1);
-                            raise_top(v0);
+                        for (int e = 4; e < 32; ++e) a[e & 3] = fmaxf(a[e & 3], __uint_as_float(x[e]));
+                        const float top = fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3]));
+                        const float over = fmaf(top, sc, -off);  // infinite at first, NaN while nothing is visible
+                        const bool raise = mine && over > RAISE;
+                        if (!__any_sync(0xffffffffu, raise)) return;
+                        float corr = 1.0f;  // a power of two: nothing is rounded again
+                        if (raise) {
+                            if (off == -INFINITY) {
+                                off = top * sc;
+                            } else {
+                                off += ceilf(over);
+                                corr = over > 126.0f ? 0.0f : __int_as_float((127 - static_cast<int>(ceilf(over))) << 23);
+                            }
                         }
-                        arrive(v1);
-                        if (k - 2 >= k0) tmem_ld_32x32b_x32(ts + 32 * (k - 2), v0);
-                        raise_top(v1);
-                    }
-                    const bool raise = mine && top > m && (m == -INFINITY || (top - m) * sc > RAISE);
-                    if (__any_sync(0xffffffffu, raise)) {
-                        const float corr = !raise ? 1.0f : m == -INFINITY ? 0.0f : exp2_approx((m - top) * sc);
-                        if (raise) m = top;
-                        l *= corr;
+                        l *= corr, sum[0] *= corr, sum[1] *= corr;
+                        tmem_wait_st();
+#pragma unroll 1
+                        for (int k = k0; k < run; ++k) {  // this tile's probabilities so far
+                            uint32_t u[16];
+                            tmem_ld_32x32b_x16(ts + 16 * k, u);
+                            tmem_wait_ld(u);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e)
+                                u[e] = pack_bf16x2(__uint_as_float(u[e] << 16) * corr,
+                                                   __uint_as_float(u[e] & 0xFFFF0000u) * corr);
+                            tmem_st_32x32b_x16(ts + 16 * k, u);
+                        }
                         if (t >= stride) {  // O holds something: the scores came after the last product
 #pragma unroll 1
                             for (int c = 0; c < HD; c += 16) {
@@ -809,31 +816,26 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                                 tmem_st_32x32b_x16(to + st * HD + c, o);
                             }
                         }
-                    }
-                    const float off = m == -INFINITY ? 0.0f : m * sc;
-                    float sum[2] = {0.0f, 0.0f};
+                    };
                     auto weigh = [&](const uint32_t (&x)[32], int run) {
+                        const float base = off == -INFINITY ? 0.0f : off;
                         uint32_t u[16];
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
-                            const float a = exp2_approx(fmaf(__uint_as_float(x[2 * e]), sc, -off));
-                            const float b = exp2_approx(fmaf(__uint_as_float(x[2 * e + 1]), sc, -off));
+                            const float a = exp2_approx(fmaf(__uint_as_float(x[2 * e]), sc, -base));
+                            const float b = exp2_approx(fmaf(__uint_as_float(x[2 * e + 1]), sc, -base));
                             u[e] = pack_bf16x2(a, b);
                             add_bf16x2(sum[0], sum[1], u[e]);
                         }
                         tmem_st_32x32b_x16(ts + 16 * run, u);  // over scores that have been read
                     };
 #pragma unroll 1
-                    for (int k = k0; k < k1; k += 2) {
-                        const bool again = k1 - k0 == 4;  // two runs are both in registers
-                        if (again) tmem_ld_32x32b_x32(ts + 32 * (k + 1), v0);
-                        weigh(v1, k);
-                        if (!single) {
-                            if (again) arrive(v0);
-                            if (k + 2 < k1) tmem_ld_32x32b_x32(ts + 32 * (k + 2), v1);
-                            weigh(v0, k + 1);
-                            if (k + 2 < k1) arrive(v1);
-                        }
+                    for (int k = k0; k < k1; ++k) {
+                        tmem_ld_32x32b_x32(ts + 32 * k, v);
+                        tmem_wait_ld();
+                        tie_regs(v);
+                        look(v, k);
+                        weigh(v, k);
                     }
                     if (copies) {  // the other copies' positions
                         const uint32_t zero[16] = {};
@@ -852,9 +854,9 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
             u_phase ^= 1;
             tc_fence_after();
 
-            // The piece's result.  Log2 units; a row whose sum is NaN keeps a
-            // finite maximum, so that no join takes it for one that saw nothing.
-            const float m2 = l != l ? 0.0f : m == -INFINITY ? -INFINITY : m * sc;
+            // The piece's result.  A row whose sum is NaN keeps a finite
+            // maximum, so that no join takes it for one that saw nothing.
+            const float m2 = l != l ? 0.0f : off;
             float top = m2, lsum = l, w0 = m2 == -INFINITY ? 0.0f : 1.0f, w1 = 0.0f;
             char *scratch = qbuf + slot * C::TILE_BYTES;  // the queries are done with
             if (!both) {  // join the streams' and copies' maxima and sums

@@ -263,6 +263,24 @@ def test_attention_variants(sess, kw):
     assert_close(st, got, want, bound)
 
 
+@pytest.mark.parametrize("rows", [1, 10, 40, 70])           # 4, 2 and 1 copies of the rows, two row tiles
+@pytest.mark.parametrize("step", [0.02, 0.5, 11.0, -3.0])   # log2 units of a position: up by little, by tiles, by runs
+def test_attention_of_climbing_scores(sess, rows, step):
+    """The maximum rises (or falls) all the way, within runs, tiles and pieces."""
+    st = ref.Step([1500], [rows], 32, seed=rows)
+    k, v = (t.cpu() for t in pools(st, 1, 64, 2))
+    q = torch.zeros((rows, 4 * 64), dtype=torch.bfloat16)
+    q[:, ::64] = 1.0                             # scores are the keys' first dim
+    for i in range(1500 + rows):
+        pg, off = st.place(0, i)
+        k[0, pg, 0, off, 0] = i * step * math.log(2)
+    out = torch.full((rows, 256), 7.0, dtype=torch.bfloat16, device=DEV)
+    got = paged.tree_attention(batch(sess, st, dev(k), dev(v)), paged.TreePlan(None, None, dev(st.plan()[2])), dev(q), 4,
+                               scale=1.0, out=out)
+    sess.synchronize()
+    assert_close(st, got.cpu().double(), *ref.attention(st, q, k[0], v[0], 4, 1.0))
+
+
 def test_attention_without_mask_is_causal(sess):
     st = ref.Step([50, 3], [40, 130], 16, parents="chain")
     assert_close(st, *run_attention(sess, st, 2, 4, 128, mask=None))
