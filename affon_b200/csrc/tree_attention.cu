@@ -175,10 +175,18 @@ struct RowMask {
     }
 };
 
+// The bounded wait, its slow part once for the whole kernel: instructions are
+// fetched from cold (all waits inlined took 1% more, short contexts or long).
+__device__ __noinline__ bool wait_slow(uint64_t *bar, uint32_t parity, volatile int *abort, unsigned *status) {
+    return mbar_wait(bar, parity, abort, status);
+}
+__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *abort, unsigned *status) {
+    return mbar_try_wait(bar, parity) || wait_slow(bar, parity, abort, status);
+}
 // A whole warp's wait, with one answer: false when it gave up, or when another
 // wait of the CTA had.
 __device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volatile int *abort, unsigned *status) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, status));
+    return __all_sync(0xffffffffu, wait(bar, parity, abort, status));
 }
 
 // A value that is the same in all lanes, known as such to the compiler.
@@ -741,7 +749,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
             const int64_t row = static_cast<int64_t>(d.first) + node;
             const RowMask mask{p.a.mask ? p.a.mask + row * p.s.mask_words : nullptr, d.n, node};
             if (both) {
-                mbar_wait(&q_empty[st], slots.parity(st) ^ 1, abort, p.status);
+                wait(&q_empty[st], slots.parity(st) ^ 1, abort, p.status);
                 load_queries<HD>(p, d, st * TILE, min(TILE, d.rows - st * TILE), 0, qbuf + st * C::TILE_BYTES, r, 128);
                 named_bar_sync(BAR_GROUP + st, 128);
                 if (r == 0) mbar_arrive(&q_full[st]);
@@ -751,7 +759,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
             const int k0 = copy << (2 - copies), k1 = (copy + 1) << (2 - copies);  // this copy's runs of 32 positions
 #pragma unroll 1
             for (int t = both ? 0 : st; t < nt; t += stride) {
-                mbar_wait(&s_full[st], s_phase, abort, p.status);
+                wait(&s_full[st], s_phase, abort, p.status);
                 s_phase ^= 1;
                 tc_fence_after();
                 uint32_t v[32];  // a run of 32 positions
@@ -850,7 +858,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[st]);
             }
-            mbar_wait(unit_done, u_phase, abort, p.status);
+            wait(unit_done, u_phase, abort, p.status);
             u_phase ^= 1;
             tc_fence_after();
 
