@@ -55,11 +55,12 @@
 // the measured copy rate.  Units of 129 to 256 rows are bound by the
 // exponentials: a warp's 128 a row (8 cycles each) hardly overlap with its
 // other instructions, 2.9 us a tile where the products take 1.2 and the
-// tile's bytes 1.4.  (8 x 8K positions under 60 drafts, 256 rows: 113 us.
+// tile's bytes 1.4.  (8 x 8K positions under 60 drafts, 256 rows: 112 us.
 // Two warps a row, turns between the streams, items of half a tile and all
 // scores in registers measured 114, 123, 126 and 119.)  Short contexts are
 // bound by latency: 4.5 us to the first scores, 2.5 to store a piece, 4 to
-// merge a unit (16 x 1000 positions, one node each: 20.4 us).
+// merge a unit (16 x 1000 positions, one node each: 19.7 us; one sequence of
+// 333: 10.9).
 #include <cuda_runtime.h>
 
 #include "common.cuh"
@@ -451,7 +452,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
             mine = pieces * p.s.kv_heads * q.units;
             int upto = static_cast<int>(mine);
 #pragma unroll 1
-            for (int o = 1; o < 32; o <<= 1) {
+            for (int o = 1; o < p.s.seqs; o <<= 1) {
                 const int v = __shfl_up_sync(0xffffffffu, upto, o);
                 if (lane >= o) upto += v;
             }
@@ -493,6 +494,9 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
             }
         }
         uint32_t queued = 0;
+        auto over = [](int a, int b) {  // a / b; few divisions have a divisor
+            return b == 1 ? a : static_cast<int>(static_cast<unsigned>(a) / static_cast<unsigned>(b));
+        };
         int tiles = 0;
         if (pos < end && !single) q = seq_tiles(p, seq), tiles = static_cast<int>(q.tiles(p.s.kv_heads));
         for (uint32_t i = 0;; ++i) {
@@ -507,7 +511,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                 if (seq >= p.s.seqs) pos = end;
             }
             if (pos < end) {
-                const int unit = at / (single ? owners : q.nt);
+                const int unit = over(at, single ? owners : q.nt);
                 d.seq = seq;
                 d.first = q.sp.first;
                 d.n = q.n;
@@ -515,8 +519,8 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                 d.nt = q.nt;
                 if (single) {
                     const int j = at - unit * owners;
-                    d.t0 = q.nt * j / owners;
-                    d.t1 = q.nt * (j + 1) / owners;
+                    d.t0 = over(q.nt * j, owners);
+                    d.t1 = over(q.nt * (j + 1), owners);
                     d.owner0 = blockIdx.x - j;
                     d.owners = owners;
                 } else {
@@ -525,7 +529,7 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                     d.owner0 = sh.owner(pos - d.t0);
                     d.owners = sh.owner(pos - d.t0 + q.nt - 1) - d.owner0 + 1;
                 }
-                d.kv = unit / q.units;
+                d.kv = over(unit, q.units);
                 d.row0 = (unit - d.kv * q.units) * ROWS;
                 d.rows = min(ROWS, q.n * p.group - d.row0);
                 at += d.t1 - d.t0;
@@ -858,6 +862,11 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[st]);
             }
+            // The rows that this thread stores: every STEP-th, from its own first.
+            constexpr int W = HD / 4, CH = W / 8, STEP = 128 / CH;
+            const int x1 = d.row0 + (both ? st * TILE : 0) + r / CH;
+            const int node1 = x1 / p.group, g1 = x1 - node1 * p.group;
+            const int dn = STEP / p.group, dg = STEP - dn * p.group;
             wait(unit_done, u_phase, abort, p.status);
             u_phase ^= 1;
             tc_fence_after();
@@ -897,7 +906,6 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
             // memory, then the warpgroup adds the copies up and stores whole
             // sectors.  Each warpgroup takes all dims of its own rows, or
             // half the dims of both streams' rows.
-            constexpr int W = HD / 4, CH = W / 8;
             const int dim0 = both ? 0 : st * (HD / 2), dim1 = both ? HD : dim0 + HD / 2;
             const int rows = both ? min(TILE, d.rows - st * TILE) : d.rows;
             const bool pair = !both && nt > 1;  // the second stream's O holds something
@@ -929,18 +937,23 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                 }
                 named_bar_sync(BAR_GROUP + st, 128);
 #pragma unroll 1
-                for (int i = r; i < rows * CH; i += 128) {
-                    const int row = i / CH, k = i % CH;  // 8 dims of a row
+                for (int row = r / CH, node = node1, g = g1; row < rows; row += STEP) {
+                    const int k = r % CH;  // 8 dims of a row
                     float o[8] = {};
-#pragma unroll 1
-                    for (int q = 0; q < 1 << copies; ++q) {
-                        const float4 x0 = *cell(row + q * (TILE >> copies), 2 * k);
-                        const float4 x1 = *cell(row + q * (TILE >> copies), 2 * k + 1);
-                        o[0] += x0.x, o[1] += x0.y, o[2] += x0.z, o[3] += x0.w;
-                        o[4] += x1.x, o[5] += x1.y, o[6] += x1.z, o[7] += x1.w;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        if (q >> copies) break;
+                        const float4 y0 = *cell(row + q * (TILE >> copies), 2 * k);
+                        const float4 y1 = *cell(row + q * (TILE >> copies), 2 * k + 1);
+                        o[0] += y0.x, o[1] += y0.y, o[2] += y0.z, o[3] += y0.w;
+                        o[4] += y1.x, o[5] += y1.y, o[6] += y1.z, o[7] += y1.w;
                     }
                     if (whole) {
-                        store8_bf16(out_row<HD>(p, d, lead + row) + c + 8 * k, o, p.a.out_pair_order);
+                        uint16_t *dst = p.a.out + (static_cast<int64_t>(d.first) + node) * p.a.ld_out +
+                                        (static_cast<int64_t>(d.kv) * p.group + g) * HD;
+                        store8_bf16(dst + c + 8 * k, o, p.a.out_pair_order);
+                        g += dg, node += dn;
+                        if (g >= p.group) g -= p.group, ++node;
                     } else {
                         float4 *dst = reinterpret_cast<float4 *>(rec + (lead + row) * HD + c + 8 * k);
                         dst[0] = make_float4(o[0], o[1], o[2], o[3]);
