@@ -52,15 +52,16 @@
 //
 // Bounds.  Units of up to 128 rows are bound by HBM once a CTA has enough
 // tiles: 64 rows on 4 x 128K positions (2.06 GB) take 315 us, 6.5 TB/s, 0.99 of
-// the measured copy rate.  Units of 129 to 256 rows are bound by the
-// exponentials: a warp's 128 a row (8 cycles each) hardly overlap with its
-// other instructions, 2.9 us a tile where the products take 1.2 and the
-// tile's bytes 1.4.  (8 x 8K positions under 60 drafts, 256 rows: 112 us.
-// Two warps a row, turns between the streams, items of half a tile and all
-// scores in registers measured 114, 123, 126 and 119.)  Short contexts are
-// bound by latency: 4.5 us to the first scores, 2.5 to store a piece, 4 to
-// merge a unit (16 x 1000 positions, one node each: 19.7 us; one sequence of
-// 333: 10.9).
+// the measured copy rate.  Units of 129 to 256 rows are bound by the turns of
+// their two streams, 2.9 us a tile: 2.0 for a row's softmax (1.1 is what the
+// exponentials of both streams' warps take, 8 cycles each) and 0.9 from its P
+// to its next scores, since P lies over S and both products come between; the
+// products alone take 1.2 and the tile's bytes 1.4.  (8 x 8K positions under
+// 60 drafts, 256 rows: 112 us.  Two warps a row, turns between the streams,
+// items of half a tile and all scores in registers measured 114, 123, 126 and
+// 119.)  Short contexts are bound by latency: 4 us to the first scores, 2.5 to
+// store a piece, 4 to merge a unit (16 x 1000 positions, one node each: 19.7
+// us; one sequence of 333: 10.9).
 #include <cuda_runtime.h>
 
 #include "common.cuh"
