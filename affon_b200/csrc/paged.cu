@@ -220,15 +220,17 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(PagedShape s, Ap
 // head) and takes the path in order.  path[i] >= i and both ascend, so a
 // place is written only after every row that is read from it has been.  The
 // last CTA of a sequence to finish writes the length, which may be the buffer
-// that the others read theirs from.
+// that the others read theirs from.  The pages of all nodes' positions are
+// read with the tree, so that a path over positions without a page (nothing
+// was appended there) is found before any of it is accepted.
 constexpr int ACCEPT_THREADS = 256;
 constexpr int MOVE_BATCH = 8;
 
 __global__ void __launch_bounds__(ACCEPT_THREADS) accept_kernel(PagedShape s, PagedStep t, AcceptArgs a,
                                                                 unsigned *counters, unsigned *status) {
     __shared__ int parent[kMaxTreeNodes], token[kMaxTreeNodes], next[kMaxTreeNodes], path[kMaxTreeNodes];
-    __shared__ int64_t from[kMaxTreeNodes], to[kMaxTreeNodes];
-    __shared__ int count_s, moves_s, last_s;
+    __shared__ int64_t place_of[kMaxTreeNodes];  // element offset of (page, position) of a node, -1: no page
+    __shared__ int count_s, first_s, last_s;
     pdl_launch_dependents();
     pdl_wait();
     const int tid = threadIdx.x, seq = blockIdx.x;
@@ -241,11 +243,16 @@ __global__ void __launch_bounds__(ACCEPT_THREADS) accept_kernel(PagedShape s, Pa
     if (tid < n) {
         const int64_t row = static_cast<int64_t>(sp.first) + tid;
         const int up = t.parents ? t.parents[row] : tid - 1;
+        const int64_t place = static_cast<int64_t>(sp.ctx) + tid;
+        const int page = t.page_table[static_cast<int64_t>(seq) * s.ld_table + (place >> s.page_shift)];
         parent[tid] = up < tid ? up : -1;
         token[tid] = a.tokens[row];
         next[tid] = a.predicted[row];
+        place_of[tid] = page >= 0 && page < s.pages
+                            ? page * s.page_stride + (place & ((1 << s.page_shift) - 1)) * s.token_stride
+                            : -1;
     }
-    if (tid == 0) moves_s = 0;
+    if (tid == 0) first_s = kMaxTreeNodes;  // the first node that moves: all behind it do
     __syncthreads();
     if (tid < 32) {
         int count = 0;
@@ -265,26 +272,14 @@ __global__ void __launch_bounds__(ACCEPT_THREADS) accept_kernel(PagedShape s, Pa
     }
     __syncthreads();
     const int count = count_s;
-    // The rows that move, as element offsets of (page, position).
-    if (tid < count && path[tid] != tid) {
-        int64_t off[2];
-        bool ok = true;
-        for (int e = 0; e < 2; ++e) {
-            const int64_t place = static_cast<int64_t>(sp.ctx) + (e ? tid : path[tid]);
-            const int page = t.page_table[static_cast<int64_t>(seq) * s.ld_table + (place >> s.page_shift)];
-            ok = ok && page >= 0 && page < s.pages;
-            off[e] = page * s.page_stride + (place & ((1 << s.page_shift) - 1)) * s.token_stride;
-        }
-        if (!ok) atomicExch(status, static_cast<unsigned>(DEV_BOUNDS));
-        from[tid] = ok ? off[0] : -1;
-        to[tid] = off[1];
-        atomicMax(&moves_s, tid + 1);
-    } else if (tid < count) {
-        from[tid] = -1;
+    // Every CTA of the sequence comes to the same answer.
+    if (__syncthreads_or(tid < count && (place_of[tid] < 0 || place_of[path[tid]] < 0))) {
+        if (tid == 0) atomicExch(status, static_cast<unsigned>(DEV_BOUNDS));
+        return;
     }
+    if (tid < count && path[tid] != tid) atomicMin(&first_s, tid);
     __syncthreads();
-    const int moves = moves_s;
-    if (moves > 0) {
+    if (first_s < count) {
         const int runs = s.head_dim >> 3;
         const int64_t items = static_cast<int64_t>(a.layers) * 2 * s.kv_heads * runs;
         for (int64_t it = static_cast<int64_t>(blockIdx.y) * ACCEPT_THREADS + tid; it < items;
@@ -295,14 +290,14 @@ __global__ void __launch_bounds__(ACCEPT_THREADS) accept_kernel(PagedShape s, Pa
             const int64_t lk = h / s.kv_heads;
             uint16_t *base = ((lk & 1) ? a.v_cache : a.k_cache) + (lk >> 1) * a.layer_stride + head * s.head_stride +
                              run * 8;
-            for (int i = 1; i < moves; i += MOVE_BATCH) {
+            for (int i = first_s; i < count; i += MOVE_BATCH) {
                 uint4 x[MOVE_BATCH];
 #pragma unroll
                 for (int e = 0; e < MOVE_BATCH; ++e)
-                    if (i + e < moves && from[i + e] >= 0) x[e] = *reinterpret_cast<const uint4 *>(base + from[i + e]);
+                    if (i + e < count) x[e] = *reinterpret_cast<const uint4 *>(base + place_of[path[i + e]]);
 #pragma unroll
                 for (int e = 0; e < MOVE_BATCH; ++e)
-                    if (i + e < moves && from[i + e] >= 0) *reinterpret_cast<uint4 *>(base + to[i + e]) = x[e];
+                    if (i + e < count) *reinterpret_cast<uint4 *>(base + place_of[i + e]) = x[e];
             }
         }
     }

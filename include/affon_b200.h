@@ -354,7 +354,9 @@ int affon_b200_argmax_finalize(affon_b200_ctx *ctx, const unsigned long long *am
  * than its page-table row) is skipped, its outputs are left as they were
  * (affon_b200_paged_plan marks its rows as padding), and the next
  * affon_b200_ctx_synchronize returns AFFON_B200_INVALID_ARG; so does a page
- * outside the pool, whose positions read as zero and are never written. */
+ * outside the pool, whose positions read as zero and are never written.
+ * affon_b200_tree_accept skips a sequence in the same way when a node that it
+ * would accept, or the place that it would move to, has no page in the pool. */
 typedef struct affon_b200_paged_desc {
     uint32_t struct_size;
     int32_t seqs;        /* 1..65536 */

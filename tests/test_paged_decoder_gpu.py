@@ -215,3 +215,21 @@ def test_pages_are_shared_out_and_overruns_reported():
         assert torch.equal(d.k_cache, k0) and int(d.ctx_lens[1]) == 62
     finally:
         d.close()
+
+
+def test_no_length_passes_nodes_without_a_page():
+    d = PagedDecoder(SMALL, 2, 6, "cuda:0", capacity=64, pages=3, page_size=16, seed=5)
+    try:
+        d.prefill([list(range(1, 15)), [1, 2, 3]])
+        d.synchronize()
+        d.set_step([3, 2], tokens=[1, 2, 3, 4, 5])           # the first one's third node is position 16
+        d._accept, d._follow = False, torch.tensor([2, 3, -1, 5, -1, 0], dtype=torch.int32, device=d.device)
+        k0 = d.k_cache.clone()
+        d.step_eager()
+        with pytest.raises(AffonError):
+            d.synchronize()
+        assert d.ctx_lens.tolist() == [14, 5]
+        free = [p for p in range(3) if p not in d._pages_of[0] + d._pages_of[1]]
+        assert torch.equal(d.k_cache[:, free], k0[:, free])
+    finally:
+        d.close()

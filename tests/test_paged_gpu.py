@@ -631,3 +631,62 @@ def test_drafted_steps_equal_plain_steps(sess):
     for s in range(seqs):
         m = min(at[s], 24)
         assert torch.equal(k2[0, s, :, :m], k1[0, s, :, :m]) and torch.equal(v2[0, s, :, :m], v1[0, s, :, :m])
+
+
+# ------------------------------------------------- accepted nodes without a page
+@pytest.mark.parametrize("layers", [0, 1, 40])               # no cache to move, one CTA a sequence, several
+@pytest.mark.parametrize("hole", ["own", "root", "target"])
+def test_accept_skips_a_sequence_whose_accepted_nodes_have_no_page(sess, layers, hole):
+    """Their keys and values were never written (or have nowhere to go), so no length may pass them: the sequence's
+    outputs and cache stay as they were, the others advance, and the next synchronize reports it."""
+    st = ref.Step([20, 14, 40], [5, 20, 6], 16, seed=3, parents="chain", pad=1)
+    st.parents[1] = np.array([-1, 0] + [1] * 17 + [18], dtype=np.int32)      # path 0, 1, 18, 19
+    tokens = np.arange(st.rows, dtype=np.int32)
+    predicted = np.full(st.rows, -7, dtype=np.int32)
+    at = int(st.cu[1])
+    for a, b in ((0, 1), (1, 18), (18, 19)):
+        predicted[at + a] = tokens[at + b]
+    predicted[at + 19] = 77
+    predicted[:4] = tokens[1:5]                              # the first sequence's whole chain
+    counts, path, nxt, lens = ref.accept(st, tokens, predicted)
+    assert counts.tolist() == [5, 4, 1] and path[1, :4].tolist() == [0, 1, 18, 19]
+    k, v = pools(st, 2, 64, 5, layers=max(1, layers))
+    k0, v0 = k.clone(), v.clone()
+    b = batch(sess, st, k, v)
+    # positions 14 and 15 lie in its first page, 16 to 31 in the second, 32 and 33 (nodes 18 and 19) in the third
+    b.page_table[1, {"own": 2, "root": 0, "target": 1}[hole]] = -1 if hole != "root" else st.pages
+    new = lambda *s: torch.full(s, 99, dtype=torch.int32, device=DEV)
+    out = paged.Accepted(new(3), new(3, st.max_nodes), new(3), b.ctx_lens)
+    if layers:
+        paged.tree_accept(b, dev(st.flat_parents()), dev(tokens), dev(predicted), out=out)
+    else:                                                    # the C call alone takes no cache
+        import ctypes
+        from affon_b200 import _lib
+        p = [dev(a) for a in (st.flat_parents(), tokens, predicted)]
+        sess.bind_stream()
+        assert _lib.lib().affon_b200_tree_accept(
+            sess._ctx, ctypes.byref(b.desc), 0, 0, b.cu_nodes.data_ptr(), *[t.data_ptr() for t in p],
+            b.page_table.data_ptr(), b.ctx_lens.data_ptr(), None, None, out.counts.data_ptr(), out.path.data_ptr(),
+            st.max_nodes, out.next_tokens.data_ptr(), out.lens.data_ptr()) == _lib.OK
+    with pytest.raises(AffonError) as err:
+        sess.synchronize()
+    assert err.value.code == "invalid_arg"
+    for got, want in ((out.counts, counts), (out.path, path), (out.next_tokens, nxt)):
+        assert got[[0, 2]].cpu().tolist() == want[[0, 2]].tolist() and (got[1] == 99).all()
+    assert b.ctx_lens.cpu().tolist() == [int(lens[0]), 14, int(lens[2])]
+    if layers:
+        counts[1] = 0                                        # nothing of it moves
+        assert torch.equal(k.cpu(), ref.move_accepted(st, k0.cpu(), path, counts))
+        assert torch.equal(v.cpu(), ref.move_accepted(st, v0.cpu(), path, counts))
+
+
+def test_accept_needs_no_page_for_what_it_does_not_accept(sess):
+    st = ref.Step([14], [20], 16, seed=3, parents=[np.array([-1] + [0] * 19, dtype=np.int32)])
+    tokens, predicted = np.arange(20, dtype=np.int32), np.full(20, 1, dtype=np.int32)
+    k, v = pools(st, 1, 64, 5)
+    b = batch(sess, st, k, v)
+    b.page_table[0, 1:] = -1                                 # positions 16 and up: nodes 2 to 19
+    a = paged.tree_accept(b, dev(st.flat_parents()), dev(tokens), dev(predicted))
+    sess.synchronize()
+    assert a.counts.tolist() == [2] and a.lens.tolist() == [16]
+    assert a.path[0, :3].tolist() == [0, 1, -1] and a.next_tokens.tolist() == [1]
