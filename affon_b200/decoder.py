@@ -43,6 +43,7 @@ stream its weights ahead of the activations it waits for); the captured 8B
 step measured 4.26 ms with it and 4.45 ms without.
 """
 import ctypes
+import itertools
 import math
 from dataclasses import dataclass
 
@@ -654,35 +655,101 @@ class PagedDecoder(QuantizedDecoder):
             self.tokens[:cu[-1]] = host(tokens).to(self.device)
 
     def _launch_step(self, finalize=True, events=None):
+        self._launch_plan()
+        super()._launch_step(finalize, events)
+
+    def _launch_plan(self):
         ptr = lambda t: t.data_ptr()
         check(self._L.affon_b200_paged_plan(self.ctx, ctypes.byref(self._paged), ptr(self.cu_nodes), ptr(self.parents),
                                             ptr(self.ctx_lens), ptr(self.page_table), ptr(self.plan.positions),
                                             ptr(self.plan.slots), ptr(self.plan.mask)), "paged_plan")
-        super()._launch_step(finalize, events)
 
     def _launch_attention(self, layer):
-        L, ctx, desc, p = self._L, self.ctx, ctypes.byref(self._paged), self.plan
+        self._launch_append(layer)
+        self._launch_tree_attention(layer)
+
+    def _launch_append(self, layer):
+        p = self.plan
         kc, vc = (t.data_ptr() for t in self._kv_layer[layer])
-        check(L.affon_b200_paged_append(ctx, desc, ctypes.byref(self._append), self.qkv.data_ptr(), self.cos.data_ptr(),
-                                        self.sin.data_ptr(), p.positions.data_ptr(), p.slots.data_ptr(),
-                                        self.q.data_ptr(), kc, vc), "paged_append")
-        check(L.affon_b200_tree_attention(ctx, desc, ctypes.byref(self._tree), self.q.data_ptr(),
-                                          self.cu_nodes.data_ptr(), self.ctx_lens.data_ptr(),
-                                          self.page_table.data_ptr(), p.mask.data_ptr(), kc, vc, self.attn.data_ptr()),
-              "tree_attention")
+        check(self._L.affon_b200_paged_append(self.ctx, ctypes.byref(self._paged), ctypes.byref(self._append),
+                                              self.qkv.data_ptr(), self.cos.data_ptr(), self.sin.data_ptr(),
+                                              p.positions.data_ptr(), p.slots.data_ptr(), self.q.data_ptr(), kc, vc),
+              "paged_append")
+
+    def _launch_tree_attention(self, layer):
+        kc, vc = (t.data_ptr() for t in self._kv_layer[layer])
+        check(self._L.affon_b200_tree_attention(self.ctx, ctypes.byref(self._paged), ctypes.byref(self._tree),
+                                                self.q.data_ptr(), self.cu_nodes.data_ptr(), self.ctx_lens.data_ptr(),
+                                                self.page_table.data_ptr(), self.plan.mask.data_ptr(), kc, vc,
+                                                self.attn.data_ptr()), "tree_attention")
 
     def _launch_finalize(self):
-        L, ctx, a = self._L, self.ctx, self.accepted
-        check(L.affon_b200_argmax_finalize(ctx, self.amax.data_ptr(), self.B, self.predicted.data_ptr(), None, 0,
-                                           self.pos.data_ptr(), self.step_ctr.data_ptr()), "finalize")
+        check(self._L.affon_b200_argmax_finalize(self.ctx, self.amax.data_ptr(), self.B, self.predicted.data_ptr(),
+                                                 None, 0, self.pos.data_ptr(), self.step_ctr.data_ptr()), "finalize")
         # Without acceptance every row is taken as it is: its token is what the row before it is held to predict.
-        expected = self.predicted if self._accept else self._follow
-        check(L.affon_b200_tree_accept(ctx, ctypes.byref(self._paged), self.cfg.layers, self.k_cache.stride(0),
-                                       self.cu_nodes.data_ptr(), self.parents.data_ptr(), self.tokens.data_ptr(),
-                                       expected.data_ptr(), self.page_table.data_ptr(), self.ctx_lens.data_ptr(),
-                                       self.k_cache.data_ptr(), self.v_cache.data_ptr(), a.counts.data_ptr(),
-                                       a.path.data_ptr(), self.max_nodes, a.next_tokens.data_ptr(), a.lens.data_ptr()),
-              "tree_accept")
+        self._launch_accept(self.predicted if self._accept else self._follow, self.accepted.lens)
+
+    def _launch_accept(self, expected, lens):
+        a = self.accepted
+        check(self._L.affon_b200_tree_accept(self.ctx, ctypes.byref(self._paged), self.cfg.layers,
+                                             self.k_cache.stride(0), self.cu_nodes.data_ptr(), self.parents.data_ptr(),
+                                             self.tokens.data_ptr(), expected.data_ptr(), self.page_table.data_ptr(),
+                                             self.ctx_lens.data_ptr(), self.k_cache.data_ptr(), self.v_cache.data_ptr(),
+                                             a.counts.data_ptr(), a.path.data_ptr(), self.max_nodes,
+                                             a.next_tokens.data_ptr(), lens.data_ptr()), "tree_accept")
+
+    # -- timing ----------------------------------------------------------------
+    def _role_launch(self, role, lins):
+        layer = itertools.cycle(range(self.cfg.layers))
+        if role == "attn":
+            return lambda: self._launch_tree_attention(next(layer))
+        if role == "append":
+            return lambda: self._launch_append(next(layer))
+        if role == "plan":
+            return self._launch_plan
+        if role == "accept":
+            lens = self._scratch_lens = torch.empty_like(self.ctx_lens)
+            return lambda: self._launch_accept(self.predicted, lens)
+        return super()._role_launch(role, lins)
+
+    def role_time_ms(self, role, reps=32):
+        """QuantizedDecoder's, with the further roles plan, append and accept (attn is the tree attention alone).  They
+        run the step that was set last, over the sequences' present lengths -- moved back, or the nodes left out, where
+        that would pass a sequence's pages -- and the cache rows that they write are put back with everything else."""
+        if role not in ("plan", "append", "attn", "accept"):
+            return super().role_time_ms(role, reps)
+        cu, lens, forest, table = (t.tolist() for t in (self.cu_nodes, self.ctx_lens, self.parents, self.page_table))
+        firsts, ctx, parents, rows = [0], [], [], []
+        for s, pages in enumerate(table):
+            held = list(itertools.takewhile(lambda page: 0 <= page < self.pages, pages))
+            room = len(held) * self.page_size
+            n = min(cu[s + 1] - cu[s], room)
+            at = max(0, min(lens[s], room - n))
+            firsts.append(firsts[-1] + n)
+            ctx.append(at)
+            parents += [min(p, i - 1) for i, p in enumerate(forest[cu[s]:cu[s] + n])]
+            rows += [(held[(at + i) // self.page_size], (at + i) % self.page_size) for i in range(n)]
+        pages, offs = torch.tensor(rows, dtype=torch.int64, device=self.device).reshape(-1, 2).unbind(1)
+        pools = (self.k_cache, self.v_cache)
+        kept = [t[:, pages, :, offs].clone() for t in pools]
+        a, p = self.accepted, self.plan
+        state = (self.cu_nodes, self.ctx_lens, self.parents, p.positions, p.slots, p.mask, self.q, a.counts, a.path,
+                 a.next_tokens)
+        saved = [t.clone() for t in state]
+        try:
+            for t, v in ((self.cu_nodes, firsts), (self.ctx_lens, ctx), (self.parents[:len(parents)], parents)):
+                t.copy_(torch.tensor(v, dtype=torch.int32))
+            self.set_stream(torch.cuda.current_stream(self.device))
+            self._launch_plan()
+            return super().role_time_ms(role, reps)
+        finally:
+            for t, v in zip(state, saved):
+                t.copy_(v)
+            for t, v in zip(pools, kept):
+                t[:, pages, :, offs] = v
+
+    def launches_by_role(self):
+        return {**super().launches_by_role(), "plan": 1, "append": self.cfg.layers, "accept": 1}
 
     def _advance(self):
         pass  # the kernels check every sequence's length against its pages

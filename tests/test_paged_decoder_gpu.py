@@ -233,3 +233,59 @@ def test_no_length_passes_nodes_without_a_page():
         assert torch.equal(d.k_cache[:, free], k0[:, free])
     finally:
         d.close()
+
+
+def state(d):
+    """Every device tensor that a decoder's next steps or its user read."""
+    a, p = d.accepted, d.plan
+    return [d.k_cache, d.v_cache, d.ctx_lens, d.cu_nodes, d.parents, d.tokens, d.predicted, d.page_table, d.h, d.ss,
+            d.xq, d.qkv, d.q, d.attn, d.act, d.amax, d.pos, d.step_ctr, p.positions, p.slots, p.mask, a.counts, a.path,
+            a.next_tokens]
+
+
+def drafted(d, nodes, rng):
+    d.set_step(nodes, np.concatenate([ref.random_forest(n, rng) for n in nodes]),
+               rng.integers(0, d.cfg.vocab, size=sum(nodes)))
+
+
+def test_timing_the_roles_leaves_the_paged_cache_as_it_was():
+    """step_breakdown between steps, with no page to spare behind the last node."""
+    d = PagedDecoder(SMALL, 3, 12, "cuda:0", capacity=128, pages=24, page_size=16, seed=5)
+    try:
+        rng = np.random.default_rng(1)
+        d.prefill([rng.integers(0, SMALL.vocab, size=n).tolist() for n in (9, 30, 2)])
+        for nodes in ([4, 4, 4], [1, 6, 0]):
+            for s, n in enumerate(nodes):
+                d.reserve(s, int(d.ctx_lens[s]) + n)
+            drafted(d, nodes, rng)
+            d.step_eager()
+            d.synchronize()
+            before = [t.clone() for t in state(d)]
+            parts = d.step_breakdown()
+            d.synchronize()                      # nothing was reported
+            for t, was in zip(state(d), before):
+                assert torch.equal(t, was)
+            assert {"plan", "append", "attn", "accept", "qkv", "embed", "finalize"} <= set(parts)
+            assert all(ms > 0 for ms, _ in parts.values())
+            assert sum(n for _, n in parts.values()) == d.launches_per_step()
+    finally:
+        d.close()
+
+
+def test_timing_the_roles_of_a_decoder_without_pages():
+    d = PagedDecoder(SMALL, 2, 4, "cuda:0", capacity=64, pages=3, page_size=16, seed=5)
+    try:
+        before = [t.clone() for t in state(d)]
+        for role in ("plan", "append", "attn", "accept"):
+            assert d.role_time_ms(role) > 0
+        d.set_step([3, 1], tokens=[1, 2, 3, 4])
+        d.reserve(0, 2)
+        after = [t.clone() for t in state(d)]
+        for role in ("plan", "append", "attn", "accept"):
+            assert d.role_time_ms(role) > 0
+        d.synchronize()
+        for t, was, now in zip(state(d), before, after):
+            assert torch.equal(t, now)
+        assert torch.equal(d.k_cache, before[0])
+    finally:
+        d.close()
