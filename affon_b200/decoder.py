@@ -567,8 +567,9 @@ class PagedDecoder(QuantizedDecoder):
     plain decoding; a chain of prompt tokens whose predictions are not compared
     (`accept=False`) fills the cache.
 
-    Each sequence can hold `capacity` positions; the pool has `pages` pages of
-    `page_size` positions, handed out by `reserve` and returned by `release`.
+    Each sequence can hold `capacity` positions, rounded up to whole pages
+    (`cap`); the pool has `pages` pages of `page_size` positions, handed out by
+    `reserve` and returned by `release`.
     The plan of a step, the rotation and append, the tree attention and the
     acceptance are the affon_b200 paged-cache kernels; everything else is the
     QuantizedDecoder's (with the same weights for the same seed)."""
@@ -581,11 +582,13 @@ class PagedDecoder(QuantizedDecoder):
             raise ValueError("page_size must be 16, 32, 64, 128 or 256")
         self.seqs, self.page_size, self.pages = seqs, page_size, pages
         self.max_nodes = min(rows, max_nodes or rows)
+        # The kernels hold a sequence to its row of the page table: the rotation tables reach as far.
+        per = -(-capacity // page_size)
+        capacity = per * page_size
         super().__init__(cfg, rows, capacity, device, seed=seed, max_steps=1, workspace_bytes=workspace_bytes,
                          overlap=overlap)
         dev = self.device
         i32 = lambda *shape: torch.zeros(shape, dtype=torch.int32, device=dev)
-        per = -(-capacity // page_size)
         self.page_table, self.ctx_lens, self.cu_nodes = i32(seqs, per) - 1, i32(seqs), i32(seqs + 1)  # -1: no page
         self.parents, self.predicted = i32(rows), i32(rows)
         words = -(-self.max_nodes // 32)

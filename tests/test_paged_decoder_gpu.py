@@ -289,3 +289,33 @@ def test_timing_the_roles_of_a_decoder_without_pages():
         assert torch.equal(d.k_cache, before[0])
     finally:
         d.close()
+
+
+def test_a_capacity_that_ends_inside_a_page():
+    """Sequences hold whole pages: steps across the capacity asked for are those of a decoder that was asked for the
+    whole page, and steps across the last page leave everything as it was."""
+    outs = []
+    for capacity in (100, 128):
+        d = PagedDecoder(SMALL, 1, 4, "cuda:0", capacity=capacity, pages=2, page_size=64, seed=5)
+        try:
+            rng = np.random.default_rng(1)
+            d.prefill([rng.integers(0, SMALL.vocab, size=99).tolist()])
+            d.set_step([3], tokens=[5, 6, 7])
+            d.step_eager()
+            d.synchronize()
+            got = [t.clone() for t in state(d)]
+            assert got[2].tolist() == [99 + int(d.accepted.counts[0])]
+            outs.append(got)
+            d.ctx_lens[0] = 126
+            k0, v0 = d.k_cache.clone(), d.v_cache.clone()
+            d.step_eager()
+            with pytest.raises(AffonError) as err:
+                d.synchronize()
+            assert err.value.code == "invalid_arg" and d.ctx_lens.tolist() == [126]
+            assert torch.equal(d.k_cache, k0) and torch.equal(d.v_cache, v0)
+            with pytest.raises(ValueError):
+                d.reserve(0, 129)
+        finally:
+            d.close()
+    for x, y in zip(*outs):
+        assert torch.equal(x, y)
