@@ -37,7 +37,11 @@
 //
 // A row's maximum is only raised when a score passes it by more than 2^8, and
 // then by a whole power of two: the sums, the tile's probabilities so far and
-// O are rescaled without another rounding, and rarely.  So a run of 32 scores
+// O are rescaled without another rounding, and rarely.  What is subtracted is a
+// whole number of log2 units, and the factor is that of the difference of the
+// old and the new one as f32 holds them, so weights from before and after a
+// raise have one base however far the scores are from zero (up to 2^30, where
+// f32 steps by 128 and a probability may leave its range).  A run of 32 scores
 // is read once, and little code does for all of it: short contexts wait for
 // instructions as much as for data (a pass for the maximum before the one for
 // the exponentials, with loads ahead, took 12.8 us instead of 11.7 for one
@@ -799,10 +803,11 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
                         float corr = 1.0f;  // a power of two: nothing is rounded again
                         if (raise) {
                             if (off == -INFINITY) {
-                                off = top * sc;
+                                off = ceilf(top * sc);
                             } else {
-                                off += ceilf(over);
-                                corr = over > 126.0f ? 0.0f : __int_as_float((127 - static_cast<int>(ceilf(over))) << 23);
+                                const float up = off + ceilf(over), by = up - off;
+                                off = up;
+                                corr = by > 126.0f ? 0.0f : __int_as_float((127 - static_cast<int>(by)) << 23);
                             }
                         }
                         l *= corr, sum[0] *= corr, sum[1] *= corr;

@@ -420,7 +420,8 @@ int affon_b200_paged_append(affon_b200_ctx *ctx, const affon_b200_paged_desc *de
  * padding rows are left as they were.  What a mask hides does not reach the
  * result, infinities and NaN included; what is visible and not finite makes
  * the results that it reaches not finite (an infinite value may become NaN;
- * a position whose score is minus infinity has no weight).  A step has at most
+ * a position whose score is minus infinity has no weight).  Scores are f32 and
+ * may be as large as 7e8 (2^30 / log2(e)) in magnitude.  A step has at most
  * 2^30 tiles of 128 positions x 256 rows of a KV head.  out must not overlap q
  * or the caches.  The launch uses the context's workspace; the lengths must
  * not change while it runs. */

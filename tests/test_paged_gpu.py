@@ -690,3 +690,75 @@ def test_accept_needs_no_page_for_what_it_does_not_accept(sess):
     sess.synchronize()
     assert a.counts.tolist() == [2] and a.lens.tolist() == [16]
     assert a.path[0, :3].tolist() == [0, 1, -1] and a.next_tokens.tolist() == [1]
+
+
+# ------------------------------------------------------- climbing and far scores
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("step", [0.02, 0.5, 11.0, -3.0])
+def test_climbing_scores_of_one_copy_in_alternate_tiles(sess, hd, step):
+    """100 query rows: one copy of the rows, whose streams take alternate tiles and rescale their own O."""
+    st = ref.Step([1500], [25], 32, seed=25)
+    k, v = (t.cpu() for t in pools(st, 1, hd, 2))
+    q = torch.zeros((25, 4 * hd), dtype=torch.bfloat16)
+    q[:, ::hd] = 1.0
+    for i in range(1525):
+        pg, off = st.place(0, i)
+        k[0, pg, 0, off, 0] = i * step * math.log(2)
+    out = torch.full((25, 4 * hd), 7.0, dtype=torch.bfloat16, device=DEV)
+    got = paged.tree_attention(batch(sess, st, dev(k), dev(v)), paged.TreePlan(None, None, dev(st.plan()[2])), dev(q), 4,
+                               scale=1.0, out=out)
+    sess.synchronize()
+    assert_close(st, got.cpu().double(), *ref.attention(st, q, k[0], v[0], 4, 1.0))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rows", [1, 10, 25, 70])            # 4, 2 and 1 copies of the rows, two row tiles
+def test_a_raise_between_far_scores_keeps_their_weights(sess, rows, hd):
+    """Scores near 2^22 log2 units, where f32 steps by 1/4 below and 1/2 above: all positions score 5592401 but one
+    5592413 at three quarters of the context, both exact in f32, times 0.75 log2 units.  Values are 1 and -1.
+
+    The weights' ratio is 2^-9 up to the rounding of 0.75 (12 * 0.75 * 2^-23 of an exponent) and exp's, so the result
+    is off by a probability's rounding to bf16 (2^-8 of sum p |v - o| = 1 - o^2) and its own."""
+    st = ref.Step([2000 + 37 * s for s in range(8)], [rows] * 8, 64, seed=rows)
+    heads, scale = 8, float(np.float32(0.75 * math.log(2)))
+    k = torch.zeros((st.pages, heads, 64, hd), dtype=torch.bfloat16)
+    v = torch.ones_like(k)
+    k[..., 0], k[..., 1], k[..., 2] = 85 * 65536, 85 * 256, 81
+    for s in range(8):
+        pg, off = st.place(s, 1500)
+        k[pg, :, off, 2], v[pg, :, off] = 93, -1
+    q = torch.zeros((st.rows, heads * 4 * hd), dtype=torch.bfloat16)
+    for d in range(3):
+        q[:, d::hd] = 1.0
+    got = paged.tree_attention(batch(sess, st, dev(k)[None], dev(v)[None]),
+                               paged.TreePlan(None, None, dev(st.plan()[2])), dev(q), heads * 4, scale=scale)
+    sess.synchronize()
+    got = got.cpu().double()
+    for s in range(8):
+        a = int(st.cu[s])
+        seen = st.ctx[s] - 1 + torch.from_numpy(ref.ancestors(st.parents[s])).sum(-1).double()
+        w = seen * 2.0 ** -9
+        want = ((w - 1) / (w + 1))[:, None]
+        tol = (2.0 ** -8 + 2.0 ** -12) * (1 - want ** 2) + 2.0 ** -8 * want.abs()
+        err = (got[a:a + rows] - want).abs()
+        assert (err <= tol).all(), float((err / tol).max())
+
+
+@pytest.mark.parametrize("far", [2.0 ** 20, -2.0 ** 26, 7.0e8, -7.0e8])
+@pytest.mark.parametrize("rows", [1, 25, 70])
+def test_equal_far_scores_give_the_mean(sess, rows, far):
+    """Up to the largest scores that are promised: every position has the same one, so the probabilities are equal
+    whatever their rounding, and the result is off by the f32 sums and its own rounding to bf16."""
+    st = ref.Step([700], [rows], 32, seed=rows)
+    k, v = (t.cpu() for t in pools(st, 1, 64, 7))
+    k.zero_()
+    k[..., 0], k[..., 1] = 85 * 256, 81
+    q = torch.zeros((rows, 4 * 64), dtype=torch.bfloat16)
+    q[:, ::64], q[:, 1::64] = 1.0, 1.0
+    scale = float(np.float32(far / (85 * 256 + 81)))
+    got = paged.tree_attention(batch(sess, st, dev(k), dev(v)), paged.TreePlan(None, None, dev(st.plan()[2])), dev(q), 4,
+                               scale=scale)
+    sess.synchronize()
+    want, _ = ref.attention(st, q, k[0], v[0], 4, 0.0)
+    mag, _ = ref.attention(st, q, k[0], v[0].abs(), 4, 0.0)
+    assert ((got.cpu().double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -14 * mag).all()
