@@ -157,7 +157,6 @@ class Session:
             check(L.affon_b200_ctx_reserve_workspace(ctx, int(workspace_bytes)), "workspace")
         self.device = device
         self.disposed = False
-        self._bound = 0  # the stream the context was created on
         self._cache = {}
 
     # -- tensors ---------------------------------------------------------
@@ -191,15 +190,10 @@ class Session:
         return exe
 
     # -- native launches ---------------------------------------------------
-    def _stream(self):
-        return torch.cuda.current_stream(self.torch_device).cuda_stream
-
     def bind_stream(self):
-        """Point the context at torch's current stream of the Session's device."""
-        raw = torch._C._cuda_getCurrentRawStream(self.ordinal)
-        if raw != self._bound:
-            check(_lib.lib().affon_b200_ctx_set_stream(self._ctx, raw))
-            self._bound = raw
+        """Point the context at torch's current stream of the Session's device (on every call: another thread's may
+        have come between)."""
+        check(_lib.lib().affon_b200_ctx_set_stream(self._ctx, torch._C._cuda_getCurrentRawStream(self.ordinal)))
 
     def launch_qmm(self, desc, x, w, s, b, y, selection=None):
         L = _lib.lib()

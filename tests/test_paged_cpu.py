@@ -175,3 +175,24 @@ def test_reference_accept_walks_the_lowest_fitting_child():
     counts, path, nxt, lens = ref.accept(st, tokens, predicted)
     assert counts.tolist() == [3] and path[0].tolist() == [0, 2, 3, -1, -1, -1]
     assert nxt.tolist() == [7] and lens.tolist() == [10]
+
+
+def test_a_session_used_by_two_streams_keeps_neither(monkeypatch):
+    """Another thread's call may come between a call's two steps, to read its stream and to set the context's: the
+    next call sets its own again."""
+    from affon_b200 import core
+    seen = []
+    streams = iter([1, 2, 1])
+    s = object.__new__(core.Session)
+    s._ctx, s.ordinal, s.disposed = None, 0, False
+
+    def set_stream(ctx, raw):
+        seen.append(raw)
+        if len(seen) == 1:
+            s.bind_stream()                                  # the other thread's whole call
+        return _lib.OK
+    monkeypatch.setattr(core._lib, "lib", lambda: SimpleNamespace(affon_b200_ctx_set_stream=set_stream))
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda ordinal: next(streams), raising=False)
+    s.bind_stream()
+    s.bind_stream()
+    assert seen == [1, 2, 1]
