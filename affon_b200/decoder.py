@@ -564,8 +564,8 @@ class PagedDecoder(QuantizedDecoder):
     model's own choices follow, and advances every sequence by it.  Afterwards
     `accepted` holds counts, path, next_tokens and lens (device tensors), and
     `predicted` the model's choice after every row.  One node per sequence is
-    plain decoding; a chain of prompt tokens whose predictions are not compared
-    (`accept=False`) fills the cache.
+    plain decoding.  `prefill` feeds prompts, whose tokens are taken whatever
+    the model predicts: to all sequences anew, or to some while others wait.
 
     Each sequence can hold `capacity` positions, rounded up to whole pages
     (`cap`); the pool has `pages` pages of `page_size` positions, handed out by
@@ -764,18 +764,22 @@ class PagedDecoder(QuantizedDecoder):
         self.ctx_lens.zero_()
         self._pos_host = 0
 
-    def prefill(self, prompts):
+    def prefill(self, prompts, keep=False):
         """Fill each sequence with its prompt (lists of tokens, one per sequence; may be empty), in steps of as many
-        rows as fit; afterwards accepted.next_tokens holds the token the model samples after a prompt's last one (for
-        the sequences whose prompt ended in the last step that fed them)."""
+        rows as fit; afterwards accepted.next_tokens holds the token the model samples after each prompt's last one
+        (-1 where there was none).  keep: a prompt goes on from what its sequence holds, and sequences without one stay
+        as they are, their next_tokens included."""
         if len(prompts) != self.seqs:
             raise ValueError(f"prefill needs {self.seqs} prompts")
-        self.reset()
+        held = self.ctx_lens.tolist() if keep else [0] * self.seqs
+        for s, prompt in enumerate(prompts):
+            if len(prompt):
+                self.reserve(s, held[s] + len(prompt))
+        if not keep:
+            self.reset()
         self._follow = torch.zeros_like(self.predicted)
         done, graph = [0] * self.seqs, self.graph
-        sampled = torch.full_like(self.accepted.next_tokens, -1)
-        for s, prompt in enumerate(prompts):
-            self.reserve(s, len(prompt))
+        sampled = self.accepted.next_tokens.clone() if keep else torch.full_like(self.accepted.next_tokens, -1)
         self._accept, self.graph = False, None
         try:
             while any(d < len(p) for d, p in zip(done, prompts)):

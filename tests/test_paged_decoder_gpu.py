@@ -319,3 +319,52 @@ def test_a_capacity_that_ends_inside_a_page():
             d.close()
     for x, y in zip(*outs):
         assert torch.equal(x, y)
+
+
+def test_a_prompt_joins_running_sequences():
+    """prefill(keep=True) feeds prompts to some sequences and leaves the others, their next tokens included; the joined
+    sequence holds, bit for bit, what it holds when it is alone."""
+    rng = np.random.default_rng(4)
+    first, second, more = (rng.integers(0, SMALL.vocab, size=n).tolist() for n in (21, 30, 7))
+    made = lambda: PagedDecoder(SMALL, 2, 8, "cuda:0", capacity=128, pages=16, page_size=16, seed=5)
+    d, alone = made(), made()
+    try:
+        d.prefill([first, []])
+        for _ in range(3):
+            d.reserve(0, int(d.ctx_lens[0]) + 1)
+            d.set_step([1, 0], tokens=[int(d.accepted.next_tokens[0])])
+            d.step_eager()
+        d.synchronize()
+        k, v = cached(d, 1, 0, 24)
+        nxt = int(d.accepted.next_tokens[0])
+        d.prefill([[], second], keep=True)
+        d.synchronize()
+        alone.prefill([[], second])
+        alone.synchronize()
+        assert d.ctx_lens.tolist() == [24, 30]
+        assert d.accepted.next_tokens.tolist() == [nxt, int(alone.accepted.next_tokens[1])]
+        for got, want in zip(cached(d, 1, 0, 24), (k, v)):
+            assert torch.equal(got, want)
+        d.prefill([[], more], keep=True)                     # a sequence's own prompt goes on, too
+        alone.prefill([[], more], keep=True)
+        d.synchronize()
+        alone.synchronize()
+        for li in range(SMALL.layers):
+            for got, want in zip(cached(d, li, 1, 37), cached(alone, li, 1, 37)):
+                assert torch.equal(got, want)
+        # what does not fit is refused before anything is lost
+        for prompts, keep in (([[1] * 129, []], False), ([[1] * 105, []], True), ([[1]], True)):
+            with pytest.raises(ValueError):
+                d.prefill(prompts, keep=keep)
+        assert d.ctx_lens.tolist() == [24, 37]
+        # captured steps go on as they were
+        d.reserve(0, 25)
+        d.reserve(1, 38)
+        d.set_step([1, 1], tokens=d.accepted.next_tokens.tolist())
+        d.capture()
+        d.replay()
+        d.synchronize()
+        assert d.ctx_lens.tolist() == [25, 38]
+    finally:
+        d.close()
+        alone.close()
