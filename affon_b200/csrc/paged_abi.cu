@@ -54,6 +54,8 @@ int check_desc(const affon_b200_paged_desc *d, afb::PagedShape *s) {
 }
 
 int check_launch(affon_b200_ctx *ctx, const char *what, const afb::DeviceGuard &guard) {
+    if (!ctx->workspace)  // its growth failed: the status word and the counters have no place
+        return fail(AFFON_B200_UNSUPPORTED, "%s: the context has no workspace", what);
     if (!guard.ok) return fail(AFFON_B200_CUDA_ERROR, "%s: cudaSetDevice(%d) failed", what, ctx->device);
     return AFFON_B200_OK;
 }

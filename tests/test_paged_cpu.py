@@ -196,3 +196,18 @@ def test_a_session_used_by_two_streams_keeps_neither(monkeypatch):
     s.bind_stream()
     s.bind_stream()
     assert seen == [1, 2, 1]
+
+
+def test_a_context_without_a_workspace_is_refused():
+    """What a failed growth of the workspace leaves: the kernels' status word and counters have no place."""
+    L = _lib.lib()
+    ctx = ctypes.cast(ctypes.create_string_buffer(4096), ctypes.c_void_p)  # a context of zeros
+    d, some = desc(), 4096                                   # buffers that are never read
+    p = ctypes.byref(d)
+    a = ctypes.byref(_lib.AppendDesc(ctypes.sizeof(_lib.AppendDesc), _lib.BF16, 0, 0, 0, 0, 256, 0, 512, 0))
+    t = ctypes.byref(_lib.TreeAttnDesc(ctypes.sizeof(_lib.TreeAttnDesc), 4, 1.0, 0, 512, 512))
+    for status in (L.affon_b200_paged_plan(ctx, p, *[some] * 7),
+                   L.affon_b200_paged_append(ctx, p, a, *[some] * 8),
+                   L.affon_b200_tree_attention(ctx, p, t, *[some] * 8),
+                   L.affon_b200_tree_accept(ctx, p, 1, 0, *[some] * 10, 4, some, some)):
+        assert status == _lib.UNSUPPORTED and "workspace" in _lib.last_error()
