@@ -61,11 +61,6 @@ def _ints(session, t, name, shape):
     return t
 
 
-def _row_stride(t):
-    """Elements between rows (a lone row has whatever stride it was given: use a dense one)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
 def _dense(t, dtype, shape, device):
     """Whether t needs no closer look (the checks of a decode step's calls are most of their host time)."""
     return (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == device
@@ -79,7 +74,7 @@ def _rows_of(session, t, name, dtypes, rows, cols, more=False):
     _tensor(session, t, name, dtypes, 2)
     _check(t.shape[0] == rows and (t.shape[1] == cols or more and t.shape[1] > cols),
            f"{name} must be [{rows}, {cols}{' or more' if more else ''}], not {list(t.shape)}")
-    return _row_stride(t)
+    return t.stride(0) if rows > 1 else cols  # a lone row's stride is never used
 
 
 def _ready(session):

@@ -211,3 +211,13 @@ def test_a_context_without_a_workspace_is_refused():
                    L.affon_b200_tree_attention(ctx, p, t, *[some] * 8),
                    L.affon_b200_tree_accept(ctx, p, 1, 0, *[some] * 10, 4, some, some)):
         assert status == _lib.UNSUPPORTED and "workspace" in _lib.last_error()
+
+
+def test_a_lone_row_needs_no_aligned_stride():
+    """The stride of a one-element axis is never used: one row may have any number of further columns."""
+    bf = torch.zeros((1, 517), dtype=torch.bfloat16)
+    assert paged._rows_of(HOST, bf, "qkv", (torch.bfloat16,), 1, 512, more=True) == 512
+    assert paged._rows_of(HOST, bf[:, :512], "q", (torch.bfloat16,), 1, 512) == 512
+    two = torch.zeros((2, 520), dtype=torch.bfloat16)
+    assert paged._rows_of(HOST, two[:, :512], "q", (torch.bfloat16,), 2, 512) == 520
+    assert paged._rows_of(HOST, two, "qkv", (torch.bfloat16,), 2, 512, more=True) == 520

@@ -762,3 +762,18 @@ def test_equal_far_scores_give_the_mean(sess, rows, far):
     want, _ = ref.attention(st, q, k[0], v[0], 4, 0.0)
     mag, _ = ref.attention(st, q, k[0], v[0].abs(), 4, 0.0)
     assert ((got.cpu().double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -14 * mag).all()
+
+
+def test_append_of_one_row_with_further_columns(sess):
+    st = ref.Step([5], [1], 16)
+    k, v = pools(st, 2, 64, 1)
+    b = batch(sess, st, k, v)
+    pos, slots, _ = st.plan()
+    p = paged.TreePlan(dev(pos), dev(slots))
+    wide = torch.randn((1, 8 * 64 + 5), device=DEV).to(torch.bfloat16)       # 517 columns: not a multiple of 16 bytes
+    q = paged.append(b, p, wide, 4, rope="none")
+    sess.synchronize()
+    pg, off = st.place(0, 5)
+    assert torch.equal(q, wide[:, :256])
+    assert torch.equal(k[0, pg, :, off].flatten(), wide[0, 256:384])
+    assert torch.equal(v[0, pg, :, off].flatten(), wide[0, 384:512])
