@@ -120,10 +120,16 @@ cudaError_t launch_qmv(const QmmArgs &a, const QmvPlan &p, void *workspace, cuda
 cudaError_t launch_resid_norm(float *h, int64_t ld_h, const float *add, int64_t ld_add, const uint16_t *gamma,
                               float eps, int M, int K, int bits, uint16_t *dst, int64_t ld_dst, cudaStream_t stream,
                               bool pdl);
-// Test hook of the split-K combine: its wait limit (0 = the default) and
-// arrivals it waits for beyond the real contributors (0 in normal use; 1
-// makes every shared block's wait run out).  Process-wide.
+// Test hook of the split-K combine and of the tree attention's merge: the wait
+// limit (0 = the default) and arrivals waited for beyond the real contributors
+// (0 in normal use; 1 makes every shared block's or unit's wait run out).
+// Process-wide.
 void qmv_set_combine_wait(uint64_t limit_ns, unsigned extra_arrivals);
+struct CombineWait {
+    uint64_t limit_ns;
+    unsigned extra_arrivals;
+};
+CombineWait qmv_combine_wait();
 
 // Decoder kernels around the quantized linears (decode.cu).
 struct DecodeAttnArgs {

@@ -1773,6 +1773,8 @@ void qmv_set_combine_wait(uint64_t limit_ns, unsigned extra_arrivals) {
     g_extra_arrivals.store(extra_arrivals);
 }
 
+CombineWait qmv_combine_wait() { return {g_arrival_wait_ns.load(), g_extra_arrivals.load()}; }
+
 template <int BITS, int MT, int NT, int CW>
 static cudaError_t launch_cfg(const CUtensorMap &wm, const CUtensorMap &sm, const CUtensorMap &bm,
                               const CUtensorMap &xm, const qmv::Params &p, const QmvPlan &plan, cudaStream_t stream,
@@ -1833,8 +1835,9 @@ cudaError_t launch_qmv(const QmmArgs &a, const QmvPlan &plan, void *workspace, c
     p.stages = plan.stages;
     p.max_slots = plan.max_slots;
     p.y_bf16 = a.y_bf16;
-    p.arrival_wait_ns = g_arrival_wait_ns.load();
-    p.extra_arrivals = g_extra_arrivals.load();
+    const CombineWait wait = qmv_combine_wait();
+    p.arrival_wait_ns = wait.limit_ns;
+    p.extra_arrivals = wait.extra_arrivals;
     if (fusion) p.f = *fusion;
     char *ws = static_cast<char *>(workspace);
     p.status = reinterpret_cast<unsigned *>(ws);

@@ -109,6 +109,7 @@ struct Params {
     int group;           // query heads per KV head
     float *partial;      // [grid][2] records
     unsigned *arrived, *done, *status;
+    CombineWait merge;   // limit of a merge's wait for the other CTAs of a unit
 };
 
 // The tiles of one sequence: kv_heads * row tiles * position tiles.
@@ -1008,8 +1009,9 @@ __global__ void __launch_bounds__(THREADS, 1) tree_attention_kernel(const __grid
             if (rows > 0) {
                 if (lane == 0) {
                     const uint64_t since = globaltimer();
-                    while (ok && *reinterpret_cast<volatile unsigned *>(&p.arrived[owner0]) != static_cast<unsigned>(k))
-                        if (*abort || globaltimer() - since > kArrivalWaitNs) {
+                    const unsigned want = static_cast<unsigned>(k) + p.merge.extra_arrivals;
+                    while (ok && *reinterpret_cast<volatile unsigned *>(&p.arrived[owner0]) != want)
+                        if (*abort || globaltimer() - since > p.merge.limit_ns) {
                             atomicExch(p.status, static_cast<unsigned>(DEV_TIMEOUT));
                             ok = false;
                         }
@@ -1153,6 +1155,7 @@ cudaError_t launch_tree_attention(const PagedShape &s, const PagedStep &t, const
     p.arrived = reinterpret_cast<unsigned *>(ws + kCounterOffset);
     p.done = p.arrived + kMaxTiles / 2;
     p.partial = reinterpret_cast<float *>(ws + kPartialOffset);
+    p.merge = qmv_combine_wait();
     // No more CTAs than tiles there can be.
     const int64_t positions = s.ld_table << s.page_shift;
     const int64_t tiles = (positions + tattn::TILE - 1) / tattn::TILE * s.kv_heads *

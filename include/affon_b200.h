@@ -132,11 +132,12 @@ int affon_b200_ctx_device(const affon_b200_ctx *ctx);
  * hold a part of the SMs (both would give up: AFFON_B200_TIMEOUT). */
 int affon_b200_ctx_set_overlap(affon_b200_ctx *ctx, int enable);
 
-/* Test hook of the decode qmv's split-K combine, process-wide: the limit of
- * its bounded wait for the other contributors of a block (0 = the default
- * 4 s) and arrivals it waits for beyond the real contributors (0 in normal
- * use; 1 makes every shared block's wait run out, so a test can check that
- * the timeout is reported and the next launch is correct). */
+/* Test hook of the decode qmv's split-K combine and of the tree attention's
+ * merge, process-wide: the limit of the bounded wait for the other
+ * contributors of a block or unit (0 = the default 4 s) and arrivals it waits
+ * for beyond the real contributors (0 in normal use; 1 makes every shared
+ * block's wait run out, so a test can check that the timeout is reported and
+ * the next launch is correct). */
 int affon_b200_debug_set_combine_wait(uint64_t limit_ns, uint32_t extra_arrivals);
 
 /* Test hook of the reassociated prefill qmm, process-wide: the most

@@ -777,3 +777,30 @@ def test_append_of_one_row_with_further_columns(sess):
     assert torch.equal(q, wide[:, :256])
     assert torch.equal(k[0, pg, :, off].flatten(), wide[0, 256:384])
     assert torch.equal(v[0, pg, :, off].flatten(), wide[0, 384:512])
+
+
+# ------------------------------------------------------------- the merge gives up
+def test_a_merge_that_gives_up_is_reported_and_the_next_call_is_right(sess):
+    """A hook makes every merge wait (20 ms) for one piece more than there is."""
+    from affon_b200 import _lib
+    st = ref.Step([3000, 64, 900], [9, 2, 64], 16, seed=6)
+    k, v = pools(st, 4, 128, 0)
+    q = torch.randn((st.rows, 16 * 128), device=DEV).to(torch.bfloat16)
+    b = batch(sess, st, k, v)
+    plan = paged.TreePlan(None, None, dev(st.plan()[2]))
+    want = paged.tree_attention(b, plan, q, 16)
+    sess.synchronize()
+    L = _lib.lib()
+    L.affon_b200_debug_set_combine_wait(20_000_000, 1)
+    try:
+        out = torch.full_like(want, 7.0)
+        paged.tree_attention(b, plan, q, 16, out=out)
+        with pytest.raises(AffonError) as err:
+            sess.synchronize()
+        assert err.value.code == "timeout"
+    finally:
+        L.affon_b200_debug_set_combine_wait(0, 0)
+    assert (out[0] == 7.0).all()                             # the long sequence's rows were to be merged
+    for _ in range(2):
+        assert torch.equal(paged.tree_attention(b, plan, q, 16), want)
+        sess.synchronize()
