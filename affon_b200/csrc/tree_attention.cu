@@ -184,8 +184,11 @@ struct RowMask {
 
 // The bounded wait, its slow part once for the whole kernel: instructions are
 // fetched from cold (all waits inlined took 1% more, short contexts or long).
+// Once another wait of the CTA has given up, none is begun: the softmax warps
+// still walk every tile of the pieces that were queued.
 __device__ __noinline__ bool wait_slow(uint64_t *bar, uint32_t parity, volatile int *abort, unsigned *status) {
-    return mbar_wait(bar, parity, abort, status);
+    if (mbar_try_wait(bar, parity)) return true;
+    return !*abort && mbar_wait(bar, parity, abort, status);
 }
 __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity, volatile int *abort, unsigned *status) {
     return mbar_try_wait(bar, parity) || wait_slow(bar, parity, abort, status);
