@@ -11,7 +11,11 @@
 // into tiles of 128 positions.  The tiles of all units, in order, are divided
 // evenly over a persistent grid of one CTA per SM: ragged lengths balance
 // without the host knowing them (they live in device memory, so a captured
-// graph follows them).  A CTA's range covers the end of one unit, whole units
+// graph follows them).  A tile counts one whatever its unit's rows, though one
+// of 129 to 256 rows takes 2.2 times as long as the others, so steps that mix
+// such units with smaller ones balance less well; and each CTA reads the
+// lengths of all sequences first, 32 at a time.
+// A CTA's range covers the end of one unit, whole units
 // and the start of another; whole units are finished in place, pieces go to
 // the workspace and the CTAs that share a unit merge it together at the end,
 // each a share of its rows, in piece order (results do not depend on timing).
@@ -55,17 +59,18 @@
 // f32.
 //
 // Bounds.  Units of up to 128 rows are bound by HBM once a CTA has enough
-// tiles: 64 rows on 4 x 128K positions (2.06 GB) take 315 us, 6.5 TB/s, 0.99 of
-// the measured copy rate.  Units of 129 to 256 rows are bound by the turns of
+// tiles: 64 rows on 4 x 128K positions (2.06 GB) take 314 us, 6.5 TB/s, 0.99 of
+// the measured copy rate (375 us in a loop of seconds, where the power cap
+// holds the SMs at 1.1 GHz).  Units of 129 to 256 rows are bound by the turns of
 // their two streams, 2.9 us a tile: 2.0 for a row's softmax (1.1 is what the
 // exponentials of both streams' warps take, 8 cycles each) and 0.9 from its P
 // to its next scores, since P lies over S and both products come between; the
 // products alone take 1.2 and the tile's bytes 1.4.  (8 x 8K positions under
-// 60 drafts, 256 rows: 112 us.  Two warps a row, turns between the streams,
+// 60 drafts, 256 rows: 110 us.  Two warps a row, turns between the streams,
 // items of half a tile and all scores in registers measured 114, 123, 126 and
 // 119.)  Short contexts are bound by latency: 4 us to the first scores, 2.5 to
-// store a piece, 4 to merge a unit (16 x 1000 positions, one node each: 19.7
-// us; one sequence of 333: 10.9).
+// store a piece, 4 to merge a unit (16 x 1000 positions, one node each: 19.2
+// us; one sequence of 333: 11.2).
 #include <cuda_runtime.h>
 
 #include "common.cuh"

@@ -572,7 +572,9 @@ class PagedDecoder(QuantizedDecoder):
     `reserve` and returned by `release`.
     The plan of a step, the rotation and append, the tree attention and the
     acceptance are the affon_b200 paged-cache kernels; everything else is the
-    QuantizedDecoder's (with the same weights for the same seed)."""
+    QuantizedDecoder's (with the same weights for the same seed).  The two do
+    not agree bit for bit: here rotated queries and probabilities enter the
+    tensor cores as bf16, there as pairs of bf16 with 16 bits."""
 
     def __init__(self, cfg, seqs, rows, device, capacity, pages, page_size=64, max_nodes=None, seed=0,
                  workspace_bytes=None, overlap=True):
